@@ -513,6 +513,104 @@ int tq_pqo_cache_read_layer(void *cache, int layer, uint8_t *k_indices, uint16_t
 int tq_pqo_cache_buffers(void *cache, int layer, uint8_t **k_indices, uint16_t **k_scales,
                          uint8_t **v_indices, uint16_t **v_scales);
 
+/* =========================================================================
+ * A serving step over a paged compressed cache (no reference counterpart:
+ * the reference's caches hold one contiguous sequence per layer).  Records
+ * live in pages of page_size tokens (a power of two, 16 to 1024) that any
+ * request can own:
+ *   codes   [num_pages][num_kv_heads][page_size][head_dim * bits / 8] u8
+ *   scales  [num_pages][num_kv_heads][page_size][head_dim / 32] f16
+ *   signs   [num_pages][num_kv_heads][page_size][head_dim / 8] u8   (TQ)
+ *   norms   [num_pages][num_kv_heads][page_size] f16                (TQ)
+ * with the record formats above (outlier_blocks 0 or all).  Row b of
+ * block_table [batch][table_width] names request b's pages in order: token t
+ * sits at offset t % page_size of page block_table[b][t / page_size].  A slot
+ * is page * page_size + offset; a slot outside [0, num_pages * page_size), -1
+ * above all, names no token.  Code and scale pools on 16-byte boundaries.
+ * ========================================================================= */
+
+/* Pages, slots and positions of one step's tokens from the requests' lengths,
+ * in request order, on the device (nothing is read back).
+ *   kv_lens [batch]: tokens that each request holds; new_lens [batch]: tokens
+ *   that it appends, 0 for none, negative: it is done, and its pages go back.
+ *   free_pages [free_capacity]: the free pages are entries 0 .. *free_count -
+ *   1, taken from the end; pages of done requests are put there first.
+ * Request b's tokens are rows starts[b] .. starts[b + 1] - 1 of the step
+ * (starts [batch + 1], the exclusive sums of the positive new_lens).  It gets
+ * them if they end at or below num_tokens and fit its table row and, where
+ * new pages are needed, all that this and the earlier requests need are free;
+ * else it gets none of them.  appended[b]: how many it got; kv_lens_out[b]:
+ * the tokens that it then holds (0 for a done one).  New pages go into
+ * block_table; slots [num_tokens] and positions [num_tokens] are written
+ * whole, -1 in rows without a token.  kv_lens_out may be kv_lens and
+ * free_count_out free_count.  batch up to 65,535, num_tokens and each
+ * new_lens up to 2^24, table_width up to 2^20. */
+int tq_paged_plan(const int *kv_lens, const int *new_lens, int batch, int *block_table,
+                  int table_width, int *free_pages, int free_capacity, const int *free_count,
+                  int page_size, int num_tokens, long long *slots, int *positions, int *starts,
+                  int *appended, int *kv_lens_out, int *free_count_out, hipStream_t stream);
+
+/* RMS norm of each query and key head, then the position rotation, in one
+ * pass: q [tokens][num_heads][head_dim] and k [tokens][num_kv_heads]
+ * [head_dim] in dtype, rows q_stride / k_stride elements apart (heads
+ * adjacent: rows of a fused projection's output), outputs in dtype likewise;
+ * an output may be its input.
+ *   y = x / sqrt(mean(x^2) + eps) * weight, weight [head_dim] in dtype (null:
+ *   no norm), each sum in f32;
+ *   the first rot_dim elements (even, 0 to head_dim) turn by positions[t] *
+ *   inv_freq[i], i < rot_dim / 2, as pairs (i, i + rot_dim / 2), or (2 i,
+ *   2 i + 1) when interleaved; the angle is formed and reduced in 64 bits.
+ * One rounding, at the output.  Rows of negative positions are left as they
+ * are.  head_dim a multiple of 32 up to 256; inv_freq f32 [rot_dim / 2].
+ * num_heads or num_kv_heads may be 0 (then its pointers are not read). */
+int tq_qk_norm_rope(const void *q, long long q_stride, const void *k, long long k_stride, int dtype,
+                    const int *positions, int tokens, int num_heads, int num_kv_heads,
+                    int head_dim, const float *inv_freq, int rot_dim, int interleaved,
+                    const void *q_weight, const void *k_weight, float eps, void *q_out,
+                    long long q_out_stride, void *k_out, long long k_out_stride,
+                    hipStream_t stream);
+
+/* Quantizes k and v [tokens][num_kv_heads][head_dim] (dtype, rows k_stride /
+ * v_stride elements apart, heads adjacent) into the records of slots
+ * [tokens], the codes and scales of tq_polar_quantize; rows whose slot names
+ * no token are skipped.  signs non-null (with norms and sign_matrix, head_dim
+ * 64, 128 or 256, outlier_blocks 0): the keys' QJL sketch too
+ * (tq_qjl_cache_sketch).  The slots that name a token are distinct. */
+int tq_paged_store(const void *k, long long k_stride, const void *v, long long v_stride, int dtype,
+                   const long long *slots, int tokens, uint8_t *k_indices, uint16_t *k_scales,
+                   uint8_t *v_indices, uint16_t *v_scales, uint8_t *signs, uint16_t *norms,
+                   const uint32_t *sign_matrix, long long num_pages, int num_kv_heads,
+                   int page_size, int head_dim, int bits, size_t outlier_blocks, int norm_mode,
+                   hipStream_t stream);
+
+/* The records of slots [tokens] back as activations: k_out and v_out
+ * [tokens][num_kv_heads][head_dim] in out_dtype (tq_polar_dequantize's
+ * values); rows whose slot names no token are left as they are. */
+int tq_paged_load(const uint8_t *k_indices, const uint16_t *k_scales, const uint8_t *v_indices,
+                  const uint16_t *v_scales, const long long *slots, int tokens, long long num_pages,
+                  int num_kv_heads, int page_size, int head_dim, int bits, size_t outlier_blocks,
+                  int norm_mode, void *k_out, void *v_out, int out_dtype, hipStream_t stream);
+
+/* Attention of one new token per request over its pages: q and out [batch]
+ * [num_heads][head_dim]; request b attends to its first kv_lens[b] tokens
+ * (device lengths, clamped to 0 .. max_kv_len <= table_width * page_size).
+ * Arguments otherwise as tq_cache_decode_attention; signs non-null selects
+ * TQ with the projection of the query formed in the launch from sign_matrix.
+ * A table entry outside [0, num_pages) holds no tokens: its positions are
+ * skipped.  A request without tokens gets zeros.  Workspace as
+ * tq_attention_workspace_size(batch, num_heads, num_kv_heads, head_dim,
+ * max_kv_len) (one call at a time per workspace). */
+int tq_paged_decode_attention(const void *q, int q_dtype, const uint8_t *k_indices,
+                              const uint16_t *k_scales, const uint8_t *v_indices,
+                              const uint16_t *v_scales, const uint8_t *signs,
+                              const uint16_t *norms, const uint32_t *sign_matrix,
+                              const int *block_table, int table_width, const int *kv_lens,
+                              int batch, int num_heads, int num_kv_heads, int head_dim, int bits,
+                              size_t outlier_blocks, int norm_mode, int page_size,
+                              long long num_pages, int max_kv_len, float softmax_scale, void *out,
+                              int out_dtype, void *workspace, size_t workspace_bytes,
+                              hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

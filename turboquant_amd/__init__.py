@@ -16,6 +16,8 @@ from ._lib import (TQ_DTYPE_BF16, TQ_DTYPE_F16, TQ_DTYPE_F32, TQ_NORM_MAXNORM, T
                    check, lib)
 from .cache import (AttendConfig, CacheConfig, DecodeOutput, Dequantized, DequantResult, Fused, PqoCache,
                     QuantNormMode, TqCache)
+from .paged import (PagedCache, PagedLayer, PagePlan, QkNormRope, paged_decode_attention, paged_load, paged_plan,
+                    paged_store, qk_norm_rope)
 
 __all__ = [
     "TurboQuantError", "lib", "pqo_quantize", "pqo_dequantize", "quant_maxnorm_batch", "dequant_batch",
@@ -24,7 +26,8 @@ __all__ = [
     "qjl_query_context", "qjl_scores", "softmax_rows", "qjl_weighted_values", "PqoCache", "AttendConfig",
     "DequantResult", "TqCache", "CacheConfig", "QuantNormMode", "DecodeOutput", "Fused", "Dequantized",
     "polar_quantize", "polar_dequantize", "cache_decode_attention", "qjl_sign_matrix", "qjl_project",
-    "qjl_cache_sketch", "qjl_logit_bias", "cache_prefill_attention",
+    "qjl_cache_sketch", "qjl_logit_bias", "cache_prefill_attention", "PagedCache", "PagedLayer", "PagePlan",
+    "QkNormRope", "paged_plan", "qk_norm_rope", "paged_store", "paged_load", "paged_decode_attention",
 ]
 
 _DT = {torch.float32: TQ_DTYPE_F32, torch.bfloat16: TQ_DTYPE_BF16, torch.float16: TQ_DTYPE_F16}

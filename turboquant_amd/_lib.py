@@ -99,6 +99,14 @@ SIGNATURES = {
     "tq_pqo_cache_memory_usage": (_sz, [_p]),
     "tq_pqo_cache_capacity": (_sz, [_p, _i]),
     "tq_pqo_cache_read_layer": (_i, [_p, _i, _p, _p, _p, _p, _p]),
+    "tq_paged_plan": (_i, [_p, _p, _i, _p, _i, _p, _i, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p]),
+    "tq_qk_norm_rope": (_i, [_p, _ll, _p, _ll, _i, _p, _i, _i, _i, _i, _p, _i, _i, _p, _p, _f, _p, _ll, _p, _ll,
+                             _p]),
+    "tq_paged_store": (_i, [_p, _ll, _p, _ll, _i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _ll, _i, _i, _i, _i, _sz, _i,
+                            _p]),
+    "tq_paged_load": (_i, [_p, _p, _p, _p, _p, _i, _ll, _i, _i, _i, _i, _sz, _i, _p, _p, _i, _p]),
+    "tq_paged_decode_attention": (_i, [_p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _sz, _i,
+                                       _i, _ll, _i, _f, _p, _i, _p, _sz, _p]),
     "tq_pqo_cache_buffers": (_i, [_p, _i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p),
                                   C.POINTER(C.c_void_p)]),
 }

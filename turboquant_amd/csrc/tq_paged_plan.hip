@@ -1,0 +1,183 @@
+// tq_paged_plan.hip -- pages, slots and positions of a serving step from the
+// requests' lengths.
+//
+// Everything is a prefix sum over the requests: the pages that done requests
+// give back, the tokens that the others bring, the pages that they need.  One
+// workgroup of 16 waves takes 1,024 requests at a time (a DPP scan in each
+// wave, the waves' totals through LDS) and carries the sums on, so the free
+// list, which every sum goes by, is read and written in order and the step
+// needs one launch.  The launch and three dependent reads (lengths, free
+// count, pages) bound it.
+#include "tq_mfma.h"
+#include "tq_paged.h"
+
+namespace {
+
+using namespace tqm;
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kMaxTokens = 1 << 24, kMaxWidth = 1 << 20;
+// A request with at most this many new pages and tokens is written by its own
+// lane, a larger one by a wave.
+constexpr int kLaneItems = 2;
+
+struct PlanArgs {
+  const int *kv_lens, *new_lens;
+  int *table, *free_pages;
+  const int *free_count;
+  long long *slots;
+  int *positions, *starts, *appended, *kv_out, *free_out;
+  int batch, width, capacity, shift, tokens;
+};
+
+// Exclusive prefix sum of v over the workgroup's threads, and their total.
+__device__ __forceinline__ long long block_prefix(int v, int *s, int lane, int wave, long long &total) {
+  const int incl = wave_incl_scan_i(v);
+  __syncthreads();  // the totals of the scan before have been read
+  if (lane == 63) s[wave] = incl;
+  __syncthreads();
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    const int t = s[w];
+    before += w < wave ? t : 0;
+    all += t;
+  }
+  total = all;
+  return before + incl - v;
+}
+
+// What a request of the current 1,024 has to write.
+struct Item {
+  int b, held, need, kv, n, start;
+  long long top;  // stack index of its first new page
+};
+
+__device__ __forceinline__ void write_page(const PlanArgs &a, const Item &it, int j) {
+  a.table[(long long)it.b * a.width + it.held + j] = a.free_pages[it.top - j];
+}
+// Token i of the request.  Its page comes from the table or the stack, not
+// from the entry that this launch writes.
+__device__ __forceinline__ void write_token(const PlanArgs &a, const Item &it, int i) {
+  const int pos = it.kv + i, pi = pos >> a.shift;
+  const int page = pi < it.held ? a.table[(long long)it.b * a.width + pi] : a.free_pages[it.top - (pi - it.held)];
+  a.slots[it.start + i] = page < 0 ? -1 : ((long long)page << a.shift) + (pos & ((1 << a.shift) - 1));
+  a.positions[it.start + i] = pos;
+}
+__device__ __forceinline__ void write_none(const PlanArgs &a, int t) {
+  a.slots[t] = -1;
+  a.positions[t] = -1;
+}
+
+__global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
+  __shared__ int s_sum[kWaves];
+  __shared__ Item s_item[kThreads];
+  __shared__ int s_items;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int page = 1 << a.shift;
+  const long long room = (long long)a.width << a.shift;
+  const int free0 = min(max(a.free_count[0], 0), a.capacity);
+  auto kv_of = [&](int b) { return max(a.kv_lens[b], 0); };
+  auto pages_of = [&](long long tokens) { return (int)min((tokens + page - 1) >> a.shift, (long long)a.width); };
+
+  // ---- done requests put their pages on the stack, in order ----
+  long long released = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    const bool done = b < a.batch && a.new_lens[b] < 0;
+    const int back = done ? pages_of(kv_of(b)) : 0;
+    if (!__syncthreads_or(back)) continue;
+    long long total;
+    const long long at = free0 + released + block_prefix(back, s_sum, lane, wave, total);
+    // a wave copies its done requests' pages one request after the other
+    for (unsigned long long m = __ballot(back > 0); m; m &= m - 1) {
+      const int l = __builtin_ctzll(m);
+      const int cnt = __builtin_amdgcn_readlane(back, l);
+      const long long to = ((long long)__builtin_amdgcn_readlane((int)(at >> 32), l) << 32) |
+                           (uint32_t)__builtin_amdgcn_readlane((int)at, l);
+      const int *row = a.table + (long long)(b0 + 64 * wave + l) * a.width;
+      for (int j = lane; j < cnt; j += 64)
+        if (to + j < a.capacity) a.free_pages[to + j] = row[j];
+    }
+    released += total;
+  }
+  const long long avail = min(free0 + released, (long long)a.capacity);
+  __syncthreads();  // the stack is whole before pages are taken from it
+
+  // ---- the others take theirs ----
+  long long start0 = 0, taken0 = 0, used = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    const bool live = b < a.batch;
+    const int kv = live ? kv_of(b) : 0, raw = live ? a.new_lens[b] : 0;
+    const int n = min(max(raw, 0), kMaxTokens);
+    long long total, all_need;
+    const long long start = start0 + block_prefix(n, s_sum, lane, wave, total);
+    start0 += total;
+    const bool has_room = (long long)kv + n <= room && start + n <= a.tokens;
+    const int held = pages_of(kv);
+    const int need = has_room ? pages_of((long long)kv + n) - held : 0;
+    const long long taken = taken0 + block_prefix(need, s_sum, lane, wave, all_need);
+    taken0 += all_need;
+    const bool fits = has_room && (need == 0 || taken + need <= avail);
+    long long got;
+    (void)block_prefix(fits ? need : 0, s_sum, lane, wave, got);
+    used += got;
+    if (tid == 0) s_items = 0;
+    __syncthreads();
+    if (live) {
+      a.starts[b] = (int)min(start, 0x7fffffffll);
+      a.appended[b] = fits ? n : 0;
+      a.kv_out[b] = raw < 0 ? 0 : (fits ? kv + n : kv);
+      const Item it{b, held, fits ? need : 0, kv, fits ? n : 0, (int)min(start, 0x7fffffffll), avail - 1 - taken};
+      if (fits && n <= kLaneItems) {
+        for (int j = 0; j < it.need; j++) write_page(a, it, j);
+        for (int i = 0; i < n; i++) write_token(a, it, i);
+      } else if (n > 0 && start < a.tokens) {
+        s_item[atomicAdd(&s_items, 1)] = fits ? it : Item{b, -1, 0, 0, (int)min((long long)n, a.tokens - start), (int)start, 0};
+      }
+    }
+    __syncthreads();
+    const int items = s_items;
+    for (int k = wave; k < items; k += kWaves) {
+      const Item it = s_item[k];
+      if (it.held < 0) {  // it does not fit: its rows hold no tokens
+        for (int i = lane; i < it.n; i += 64) write_none(a, it.start + i);
+        continue;
+      }
+      for (int j = lane; j < it.need; j += 64) write_page(a, it, j);
+      for (int i = lane; i < it.n; i += 64) write_token(a, it, i);
+    }
+  }
+  if (tid == 0) {
+    a.starts[a.batch] = (int)min(start0, 0x7fffffffll);
+    a.free_out[0] = (int)(avail - used);
+  }
+  for (long long t = start0 + tid; t < a.tokens; t += kThreads) write_none(a, (int)t);
+}
+
+}  // namespace
+
+extern "C" int tq_paged_plan(const int *kv_lens, const int *new_lens, int batch, int *block_table, int table_width,
+                             int *free_pages, int free_capacity, const int *free_count, int page_size, int num_tokens,
+                             long long *slots, int *positions, int *starts, int *appended, int *kv_lens_out,
+                             int *free_count_out, hipStream_t stream) {
+  const int shift = tqh::page_shift(page_size);
+  if (shift < 0)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "page_size %d is no power of two from 16 to 1024", page_size);
+  if (batch < 0 || batch > 65535) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "batch %d outside 0 to 65,535", batch);
+  if (num_tokens < 0 || num_tokens > kMaxTokens)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "num_tokens %d outside 0 to 2^24", num_tokens);
+  if (table_width < 0 || table_width > kMaxWidth || (long long)table_width << shift > 0x7fffffffll)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "table_width %d: at most 2^20 pages and 2^31 - 1 tokens a request",
+                     table_width);
+  if (free_capacity < 0) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "negative free_capacity");
+  if (!starts || !free_count || !free_count_out || (free_capacity && !free_pages) ||
+      (batch && (!kv_lens || !new_lens || !appended || !kv_lens_out || (table_width && !block_table))) ||
+      (num_tokens && (!slots || !positions)))
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "null pointer");
+  PlanArgs a{kv_lens, new_lens, block_table, free_pages, free_count, slots, positions, starts, appended, kv_lens_out,
+             free_count_out, batch, table_width, free_capacity, shift, num_tokens};
+  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+  return tqh::check_launch("paged_plan_kernel");
+}

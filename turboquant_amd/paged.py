@@ -1,0 +1,343 @@
+"""A serving step over a paged compressed cache: the pages, slots and positions
+of a step's tokens from the requests' lengths (`paged_plan`), the norm of each
+query and key head with the position rotation (`qk_norm_rope`), keys and
+values into and out of their pages (`paged_store`, `paged_load`), attention of
+one new token per request (`paged_decode_attention`), and `PagedCache`, which
+runs them together.
+
+Everything is queued on the current stream of the current device, where all
+tensors of a call have to be; nothing is read back to the host, so a step can
+be captured into a graph.  Layouts: include/turboquant_amd.h.
+"""
+from __future__ import annotations
+
+from typing import List, NamedTuple, Optional, Tuple
+
+import torch
+
+from ._lib import TQ_NORM_MAXNORM, TQ_OUTLIER_ALL, check, lib
+from .cache import _DT, DEFAULT_QJL_SEED, CacheConfig, _cur_device, _stream
+
+
+def _device() -> int:
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
+def _ptr(t: torch.Tensor, dtype: torch.dtype, shape, what: str) -> int:
+    """The address of a contiguous tensor of this type and shape on the current device."""
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{what} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    dev = t.get_device()
+    if dev < 0 or dev != _device():
+        raise ValueError(f"{what} must be on the current device")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, what: str) -> Tuple[int, int]:
+    """Address and row stride (elements) of t [tokens, heads, head_dim], heads adjacent."""
+    n, h, d = t.shape
+    if t.dtype not in _DT:
+        raise ValueError(f"{what} must be f32/bf16/f16")
+    dev = t.get_device()
+    if dev < 0 or dev != _device():
+        raise ValueError(f"{what} must be on the current device")
+    if (t.stride(2) != 1 and d > 1) or (t.stride(1) != d and h > 1):
+        raise ValueError(f"{what}'s heads must be adjacent (strides {t.stride()} of {list(t.shape)})")
+    return t.data_ptr(), t.stride(0) if n > 1 else h * d
+
+
+class PagedLayer:
+    """One layer's pages: codes u8 [num_pages, num_kv_heads, page_size,
+    head_dim * bits / 8] and scales int16 (f16 bits) [..., head_dim / 32] of
+    keys and values; for TQ records also the keys' signs u8 [..., head_dim / 8]
+    and norms int16 [num_pages, num_kv_heads, page_size].  The shapes are
+    checked here, once."""
+
+    __slots__ = ("k_idx", "k_sc", "v_idx", "v_sc", "signs", "norms", "num_pages", "num_kv_heads", "page_size",
+                 "head_dim", "packed_dim", "device", "_ptrs", "_sketch")
+
+    def __init__(self, k_idx: torch.Tensor, k_sc: torch.Tensor, v_idx: torch.Tensor, v_sc: torch.Tensor,
+                 signs: Optional[torch.Tensor] = None, norms: Optional[torch.Tensor] = None):
+        if k_idx.dim() != 4 or k_sc.dim() != 4:
+            raise ValueError("pools must be [num_pages, num_kv_heads, page_size, bytes or blocks]")
+        base = k_idx.shape[:3]
+        self.num_pages, self.num_kv_heads, self.page_size = base
+        self.packed_dim, self.head_dim = k_idx.shape[3], 32 * k_sc.shape[3]
+        self.k_idx, self.k_sc, self.v_idx, self.v_sc, self.signs, self.norms = k_idx, k_sc, v_idx, v_sc, signs, norms
+        idx, sc = (*base, self.packed_dim), (*base, self.head_dim // 32)
+        self.device = k_idx.get_device()
+        self._ptrs = (_ptr(k_idx, torch.uint8, idx, "k_idx"), _ptr(k_sc, torch.int16, sc, "k_sc"),
+                      _ptr(v_idx, torch.uint8, idx, "v_idx"), _ptr(v_sc, torch.int16, sc, "v_sc"))
+        self._sketch = (None, None)
+        if (signs is None) != (norms is None):
+            raise ValueError("signs and norms come together")
+        if signs is not None:
+            self._sketch = (_ptr(signs, torch.uint8, (*base, self.head_dim // 8), "signs"),
+                            _ptr(norms, torch.int16, base, "norms"))
+
+    @staticmethod
+    def empty(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, bits: int, qjl: bool = False,
+              device="cuda") -> "PagedLayer":
+        """Zeroed pages."""
+        base = (num_pages, num_kv_heads, page_size)
+
+        def make(width, dtype):
+            return torch.zeros((*base, width), dtype=dtype, device=device)
+
+        pools = [make(w, t) for _ in range(2) for w, t in ((head_dim * bits // 8, torch.uint8),
+                                                           (head_dim // 32, torch.int16))]
+        sketch = (make(head_dim // 8, torch.uint8), torch.zeros(base, dtype=torch.int16, device=device)) if qjl else ()
+        return PagedLayer(*pools, *sketch)
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k_idx, self.k_sc, self.v_idx, self.v_sc, self.signs,
+                                                          self.norms) if t is not None)
+
+    def _check(self, bits: int, sign_matrix: Optional[torch.Tensor]):
+        """(signs, norms, sign matrix) addresses of a call; a sign matrix selects TQ."""
+        if self.device != _device():
+            raise ValueError("the layer's pages must be on the current device")
+        if 8 * self.packed_dim != self.head_dim * bits:
+            raise ValueError(f"the layer holds records of {self.packed_dim} bytes, not {bits}-bit ones of head_dim "
+                             f"{self.head_dim}")
+        if sign_matrix is None:
+            return None, None, None
+        if self.signs is None:
+            raise ValueError("a sign matrix needs pages with signs and norms")
+        words = self.head_dim * self.head_dim // 32
+        return (*self._sketch, _ptr(sign_matrix, torch.int32, (words,), "sign_matrix"))
+
+
+class PagePlan(NamedTuple):
+    """One step's tokens: slots int64 [num_tokens] and positions int32
+    [num_tokens] (-1 in rows without a token), starts int32 [batch + 1] (request
+    b's rows are starts[b] .. starts[b + 1] - 1), appended int32 [batch] (tokens
+    that each request got: all of its own, or none where they do not fit),
+    kv_lens int32 [batch] and free_count int32 [1] after the step."""
+    slots: torch.Tensor
+    positions: torch.Tensor
+    starts: torch.Tensor
+    appended: torch.Tensor
+    kv_lens: torch.Tensor
+    free_count: torch.Tensor
+
+
+def paged_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+               free_count: torch.Tensor, page_size: int, num_tokens: int, kv_lens_out: Optional[torch.Tensor] = None,
+               free_count_out: Optional[torch.Tensor] = None) -> PagePlan:
+    """Pages, slots and positions of one step's tokens from the requests'
+    lengths.  kv_lens, new_lens int32 [batch] (new_lens < 0: the request is done
+    and its pages go back), block_table int32 [batch, width] and free_pages
+    int32 [capacity] (written), free_count int32 [1].  kv_lens_out and
+    free_count_out may be the inputs; new tensors by default."""
+    if kv_lens.dim() != 1 or block_table.dim() != 2 or free_pages.dim() != 1:
+        raise ValueError("kv_lens [batch], block_table [batch, width] and free_pages [capacity] are expected")
+    b, i32, dev = kv_lens.shape[0], torch.int32, kv_lens.device
+    width, cap = block_table.shape[1], free_pages.shape[0]
+    ins = (_ptr(kv_lens, i32, (b,), "kv_lens"), _ptr(new_lens, i32, (b,), "new_lens"),
+           _ptr(block_table, i32, (b, width), "block_table"), _ptr(free_pages, i32, (cap,), "free_pages"),
+           _ptr(free_count, i32, (1,), "free_count"))
+    if num_tokens < 0:
+        raise ValueError("num_tokens must not be negative")
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    positions, starts, appended = torch.empty(num_tokens + 2 * b + 1, dtype=i32, device=dev).split(
+        (num_tokens, b + 1, b))
+    if kv_lens_out is None:
+        kv_lens_out = torch.empty_like(kv_lens)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    check(lib.tq_paged_plan(ins[0], ins[1], b, ins[2], width, ins[3], cap, ins[4], page_size, num_tokens,
+                            slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), appended.data_ptr(),
+                            _ptr(kv_lens_out, i32, (b,), "kv_lens_out"),
+                            _ptr(free_count_out, i32, (1,), "free_count_out"), _stream()))
+    return PagePlan(slots, positions, starts, appended, kv_lens_out, free_count_out)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+    """RMS norm of each head (none where its weight is None), then the position
+    rotation of its first 2 * len(inv_freq) elements.  q [tokens, heads,
+    head_dim] and k [tokens, kv_heads, head_dim] of one type, rows at any stride
+    (views of a fused projection); positions int32 [tokens], rows of negative
+    ones left as they are in the outputs; inv_freq f32 [rot_dim / 2].  Returns
+    (q, k) in new contiguous tensors, or `out` (which may be (q, k))."""
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype:
+        raise ValueError("q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] of one type are expected")
+    t, h, d = q.shape
+    if out is None:
+        out = torch.empty((t, h, d), dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo, ko = out
+    if qo.shape != q.shape or ko.shape != k.shape or qo.dtype != q.dtype or ko.dtype != k.dtype:
+        raise ValueError("out must have q's and k's shapes and type")
+    (qp, qs), (kp, ks), (qop, qos), (kop, kos) = _rows(q, "q"), _rows(k, "k"), _rows(qo, "out[0]"), _rows(ko, "out[1]")
+    wq = None if q_weight is None else _ptr(q_weight, q.dtype, (d,), "q_weight")
+    wk = None if k_weight is None else _ptr(k_weight, q.dtype, (d,), "k_weight")
+    check(lib.tq_qk_norm_rope(qp, qs, kp, ks, _DT[q.dtype], _ptr(positions, torch.int32, (t,), "positions"), t, h,
+                              k.shape[1], d, _ptr(inv_freq, torch.float32, (inv_freq.numel(),), "inv_freq"),
+                              2 * inv_freq.numel(), 1 if interleaved else 0, wq, wk, eps, qop, qos, kop, kos,
+                              _stream()))
+    return qo, ko
+
+
+def paged_store(layer: PagedLayer, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bits: int,
+                outlier_blocks: int = TQ_OUTLIER_ALL, norm_mode: int = TQ_NORM_MAXNORM,
+                sign_matrix: Optional[torch.Tensor] = None) -> None:
+    """Quantizes k and v [tokens, num_kv_heads, head_dim] (rows at any stride)
+    into the records of slots int64 [tokens]; rows whose slot is outside the
+    pages are skipped, the others' slots are distinct.  sign_matrix: TQ records,
+    whose keys are sketched too."""
+    t = slots.shape[0]
+    shape = (t, layer.num_kv_heads, layer.head_dim)
+    if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
+        raise ValueError(f"k and v must be {list(shape)} of one type, got {list(k.shape)} and {list(v.shape)}")
+    sg, nm, rm = layer._check(bits, sign_matrix)
+    (kp, ks), (vp, vs) = _rows(k, "k"), _rows(v, "v")
+    ki, ksc, vi, vsc = layer._ptrs
+    check(lib.tq_paged_store(kp, ks, vp, vs, _DT[k.dtype], _ptr(slots, torch.int64, (t,), "slots"), t, ki, ksc, vi,
+                             vsc, sg, nm, rm, layer.num_pages, layer.num_kv_heads, layer.page_size, layer.head_dim,
+                             bits, outlier_blocks, norm_mode, _stream()))
+
+
+def paged_load(layer: PagedLayer, slots: torch.Tensor, bits: int, outlier_blocks: int = TQ_OUTLIER_ALL,
+               norm_mode: int = TQ_NORM_MAXNORM, out_dtype: torch.dtype = torch.float32,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+    """The records of slots int64 [tokens] as activations: (k, v) [tokens,
+    num_kv_heads, head_dim] in out_dtype, or into `out`; rows whose slot is
+    outside the pages are left as they are."""
+    t = slots.shape[0]
+    shape = (t, layer.num_kv_heads, layer.head_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=slots.device), torch.empty(shape, dtype=out_dtype,
+                                                                                    device=slots.device)
+    k, v = out
+    if k.dtype not in _DT:
+        raise ValueError("out must be f32/bf16/f16")
+    layer._check(bits, None)
+    check(lib.tq_paged_load(*layer._ptrs, _ptr(slots, torch.int64, (t,), "slots"), t, layer.num_pages,
+                            layer.num_kv_heads, layer.page_size, layer.head_dim, bits, outlier_blocks, norm_mode,
+                            _ptr(k, k.dtype, shape, "out[0]"), _ptr(v, k.dtype, shape, "out[1]"), _DT[k.dtype],
+                            _stream()))
+    return k, v
+
+
+def paged_decode_attention(q: torch.Tensor, layer: PagedLayer, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                           bits: int, max_kv_len: int, softmax_scale: float, workspace,
+                           outlier_blocks: int = TQ_OUTLIER_ALL, norm_mode: int = TQ_NORM_MAXNORM,
+                           sign_matrix: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per request: q [batch, heads, head_dim] over
+    the first kv_lens[b] (int32, at most max_kv_len) tokens of the pages in row
+    b of block_table (int32 [batch, width]).  sign_matrix: TQ records, with the
+    QJL correction of the logits.  workspace: an AttentionWorkspace of at least
+    this batch, heads and max_kv_len; one call at a time uses it.  Returns
+    [batch, heads, head_dim] in out_dtype (q's by default)."""
+    b, h, d = q.shape
+    if d != layer.head_dim or block_table.dim() != 2:
+        raise ValueError(f"q [batch, heads, {layer.head_dim}] and block_table [batch, width] are expected")
+    width = block_table.shape[1]
+    if out is None:
+        out = torch.empty((b, h, d), dtype=out_dtype or q.dtype, device=q.device)
+    if q.dtype not in _DT or out.dtype not in _DT:
+        raise ValueError("q and out must be f32/bf16/f16")
+    sg, nm, rm = layer._check(bits, sign_matrix)
+    check(lib.tq_paged_decode_attention(
+        _ptr(q, q.dtype, (b, h, d), "q"), _DT[q.dtype], *layer._ptrs, sg, nm, rm,
+        _ptr(block_table, torch.int32, (b, width), "block_table"), width, _ptr(kv_lens, torch.int32, (b,), "kv_lens"),
+        b, h, layer.num_kv_heads, d, bits, outlier_blocks, norm_mode, layer.page_size, layer.num_pages, max_kv_len,
+        softmax_scale, _ptr(out, out.dtype, (b, h, d), "out"), _DT[out.dtype],
+        _ptr(workspace.buf, torch.uint8, (workspace.nbytes,), "workspace"), workspace.nbytes, _stream()))
+    return out
+
+
+class QkNormRope(NamedTuple):
+    """The norm and rotation of a layer's heads (`qk_norm_rope`)."""
+    inv_freq: torch.Tensor
+    q_weight: Optional[torch.Tensor] = None
+    k_weight: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+    interleaved: bool = False
+
+
+class PagedCache:
+    """Pages of every layer for up to max_requests requests of up to
+    max_kv_len tokens, with the block table and the free list on the device.
+    The layers share one table: page p of a layer holds the same tokens in all.
+
+        plan = cache.plan(new_lens, num_tokens)          # once a step
+        out = cache.step(layer, plan, q, k, v, scale, rope)   # decode, each layer
+
+    Calls are ordered on one stream; graphs captured from them share the cache
+    and its workspace, and are replayed in order."""
+
+    def __init__(self, config: CacheConfig, num_pages: int, max_requests: int, max_kv_len: int, page_size: int = 64,
+                 qjl: bool = False, device="cuda"):
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError(f"page_size {page_size} is no power of two from 16 to 1024")
+        if qjl and config.outlier_blocks != 0:
+            raise ValueError("the QJL sketch needs outlier_blocks 0")
+        if num_pages <= 0 or max_requests <= 0 or max_kv_len <= 0:
+            raise ValueError("num_pages, max_requests and max_kv_len must be positive")
+        self.config, self.page_size, self.max_requests = config, page_size, max_requests
+        self.layers: List[PagedLayer] = [
+            PagedLayer.empty(num_pages, page_size, config.num_kv_heads, config.head_dim, config.bits, qjl, device)
+            for _ in range(config.num_layers)]
+        width = -(-max_kv_len // page_size)
+        self.max_kv_len = width * page_size
+        self.block_table = torch.full((max_requests, width), -1, dtype=torch.int32, device=device)
+        self.kv_lens = torch.zeros(max_requests, dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(num_pages, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+        self.sign_matrix = None
+        if qjl:
+            from . import qjl_sign_matrix
+            self.sign_matrix = qjl_sign_matrix(config.head_dim, DEFAULT_QJL_SEED, device)
+        self._ws = None
+
+    def plan(self, new_lens: torch.Tensor, num_tokens: int) -> PagePlan:
+        """One step's pages and slots (`paged_plan`); the cache's lengths, table
+        and free list move on.  A request whose tokens would pass max_kv_len's
+        pages, or find no pages, gets none of them (appended is 0)."""
+        return paged_plan(self.kv_lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size,
+                          num_tokens, kv_lens_out=self.kv_lens, free_count_out=self.free_count)
+
+    def _mode(self):
+        return self.config.bits, self.config.outlier_blocks, int(self.config.norm_mode)
+
+    def store(self, layer: int, plan: PagePlan, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The step's keys and values [num_tokens, num_kv_heads, head_dim] into their pages."""
+        paged_store(self.layers[layer], plan.slots, k, v, *self._mode(), sign_matrix=self.sign_matrix)
+
+    def load(self, layer: int, slots: torch.Tensor, out_dtype: torch.dtype = torch.float32):
+        """Records back as activations (`paged_load`)."""
+        return paged_load(self.layers[layer], slots, *self._mode(), out_dtype=out_dtype)
+
+    def attend(self, layer: int, q: torch.Tensor, softmax_scale: float,
+               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """q [max_requests, heads, head_dim], a row per request, over all of its tokens."""
+        if q.dim() != 3 or q.shape[0] != self.max_requests:
+            raise ValueError(f"q must be [{self.max_requests}, heads, head_dim]")
+        if self._ws is None or self._ws.shape[1] < q.shape[1]:
+            from . import AttentionWorkspace
+            self._ws = AttentionWorkspace(self.max_requests, q.shape[1], self.config.num_kv_heads,
+                                          self.config.head_dim, self.max_kv_len, q.device)
+        bits, outlier_blocks, norm_mode = self._mode()
+        return paged_decode_attention(q, self.layers[layer], self.block_table, self.kv_lens, bits, self.max_kv_len,
+                                      softmax_scale, self._ws, outlier_blocks, norm_mode, self.sign_matrix, out_dtype)
+
+    def step(self, layer: int, plan: PagePlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+             softmax_scale: float, rope: Optional[QkNormRope] = None) -> torch.Tensor:
+        """A decode step of a layer: norm and rotation of q and k [num_tokens,
+        heads, head_dim], the new records, and the attention of each request's
+        last token: [max_requests, heads, head_dim].  Rows of requests that
+        bring no token in this step hold nothing of use."""
+        if rope is not None:
+            q, k = qk_norm_rope(q, k, plan.positions, *rope)
+        self.store(layer, plan, k, v)
+        rows = (plan.starts[1:] - 1).clamp_(0, max(q.shape[0] - 1, 0))
+        return self.attend(layer, q.index_select(0, rows), softmax_scale)
+
+    def memory_usage(self) -> int:
+        return sum(layer.nbytes() for layer in self.layers)
