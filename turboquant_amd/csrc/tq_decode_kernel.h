@@ -1403,8 +1403,10 @@ void launch_stream_k(AttnArgs &a, dim3 grid, hipStream_t st, int len_hint, tqh::
     constexpr auto kernel = decltype(k)::value;
     if (a.bal_nwg < 0) {
       // balanced split: as many workgroups as the compute units hold at once,
-      // at most one per task
-      a.bal_nwg = (int)min((long long)-a.bal_nwg, (long long)resident_workgroups<kernel, C::THREADS>() * device_cus());
+      // at most one per task and at least one per (sequence, KV head) pair
+      const long long pairs = (long long)a.bal_batch * a.bal_ny;
+      a.bal_nwg = (int)min((long long)-a.bal_nwg,
+                           max((long long)resident_workgroups<kernel, C::THREADS>() * device_cus(), pairs));
       grid = dim3((unsigned)a.bal_nwg, 1u, 1u);
     }
     hipLaunchKernelGGL(kernel, grid, dim3(C::THREADS), 0, st, a.k_idx, a.v_idx, a.k_sc, a.v_sc, a.seq_stride,
