@@ -114,6 +114,18 @@ struct AppendArgs {
 };
 struct NoAppend {};
 
+// Records in pages: row b of the table holds sequence b's pages in order; the
+// record of offset o of page p of KV head g is (p num_kv_heads + g) 2^shift + o.
+struct PageArgs {
+  const int *table;
+  int width;
+  int shift;
+  int num_pages;
+};
+// Sequences of a balanced split: one a lane, over pages four.
+template <bool PAGED>
+constexpr int kBalSeqs = PAGED ? 256 : 64;
+
 // Query element as stored (f32 bits or a 16-bit pattern), converted
 // separately so that the wait for the load lands at the first use.
 __device__ __forceinline__ float q_value(uint32_t bits, int qt) {
@@ -423,9 +435,10 @@ inline int store_token_apart(const tqh::AppendToken &t, AttnArgs &a, hipStream_t
 // grid.x are set from the launched configuration.  INLINE: the last
 // workgroup of a (sequence, KV head) merges the split-K partials; else the
 // caller launches stream_merge_kernel after it.  ap: a token to store before
-// attending (INLINE only; its status in ap->rc).  Defined in the
-// tq_attention_k<BITS>_<mode>.hip units.
-template <int BITS, int MODE, bool INLINE>
-void launch_stream_bm(AttnArgs &a, int nqb, int hg, dim3 grid, hipStream_t st, tqh::AppendToken *ap);
+// attending (INLINE only; its status in ap->rc), or the pages that hold the
+// records (PageArgs).  Defined in the tq_attention_k<BITS>_<mode>.hip and
+// tq_paged_k<BITS>_<mode>.hip units.
+template <int BITS, int MODE, bool INLINE, class X>
+void launch_stream_bm(AttnArgs &a, int nqb, int hg, dim3 grid, hipStream_t st, X *ap);
 
 }  // namespace tqa

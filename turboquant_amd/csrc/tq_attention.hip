@@ -1,9 +1,9 @@
 // tq_attention.hip -- fused decode attention over the compressed cache:
 // the launch configuration of the streaming decode kernel
 // (tq_decode_kernel.h), the split-K workspace (layout, header, counters),
-// and the C-ABI entry points (the batched cache decode, the reference ABI's
-// tq_fused_attention, and the allocation-free variant over a per-device
-// static scratch array).
+// and the C-ABI entry points (the batched cache decode, the decode over
+// pages, the reference ABI's tq_fused_attention, and the allocation-free
+// variant over a per-device static scratch array).
 //
 // The kernel reads every compressed byte once for all the query heads of a
 // KV head (GQA sharing), scores the keys against the rotated query without
@@ -13,6 +13,7 @@
 // them, inverse-rotates and writes the output, then re-arms the counter, so
 // one launch does the whole decode.
 #include "tq_attention.h"
+#include "tq_paged.h"
 
 #include <mutex>
 
@@ -143,23 +144,24 @@ AttnArgs base_args() {
 
 // grid: (-, num_kv_heads, batch); the chunk count (grid.x), a.nr / a.ngroups
 // and a.chunk are set here from the launched configuration
-template <bool INLINE>
-int launch_stream(AttnArgs &a, int bits, int mode, int head_dim, dim3 grid, hipStream_t st,
-                  tqh::AppendToken *ap = nullptr) {
+template <bool INLINE, class X = tqh::AppendToken>
+int launch_stream(AttnArgs &a, int bits, int mode, int head_dim, dim3 grid, hipStream_t st, X *ap = nullptr) {
   const int hg = stream_hg(a.nr);
   a.ngroups = (a.nr + hg - 1) / hg;
   grid.y *= (unsigned)a.ngroups;
   const int nqb = head_dim / 32;
   if (bits == 3) {
-    if (mode == kModePqo) launch_stream_bm<3, kModePqo, INLINE>(a, nqb, hg, grid, st, ap);
-    else if (mode == kModePq) launch_stream_bm<3, kModePq, INLINE>(a, nqb, hg, grid, st, ap);
-    else launch_stream_bm<3, kModeTq, INLINE>(a, nqb, hg, grid, st, ap);
+    if (mode == kModePqo) launch_stream_bm<3, kModePqo, INLINE, X>(a, nqb, hg, grid, st, ap);
+    else if (mode == kModePq) launch_stream_bm<3, kModePq, INLINE, X>(a, nqb, hg, grid, st, ap);
+    else launch_stream_bm<3, kModeTq, INLINE, X>(a, nqb, hg, grid, st, ap);
   } else {
-    if (mode == kModePqo) launch_stream_bm<4, kModePqo, INLINE>(a, nqb, hg, grid, st, ap);
-    else if (mode == kModePq) launch_stream_bm<4, kModePq, INLINE>(a, nqb, hg, grid, st, ap);
-    else launch_stream_bm<4, kModeTq, INLINE>(a, nqb, hg, grid, st, ap);
+    if (mode == kModePqo) launch_stream_bm<4, kModePqo, INLINE, X>(a, nqb, hg, grid, st, ap);
+    else if (mode == kModePq) launch_stream_bm<4, kModePq, INLINE, X>(a, nqb, hg, grid, st, ap);
+    else launch_stream_bm<4, kModeTq, INLINE, X>(a, nqb, hg, grid, st, ap);
   }
-  if (ap && ap->rc) return ap->rc;
+  if constexpr (std::is_same_v<X, tqh::AppendToken>) {
+    if (ap && ap->rc) return ap->rc;
+  }
   return tqh::check_launch("stream_decode_kernel");
 }
 int launch_stream_merge(const AttnArgs &a, int head_dim, dim3 grid, hipStream_t st) {
@@ -226,6 +228,18 @@ struct DecodeWs {
   size_t part_bytes = 0;
   int pairs = 0;
 };
+
+// The split-K fields of a launch over `pairs` (sequence, KV head) pairs.
+void set_workspace(AttnArgs &a, const WsLayout &w, const DecodeWs &d, long long pairs) {
+  a.po = reinterpret_cast<float *>(d.base + w.po);
+  a.pm = reinterpret_cast<float *>(d.base + w.pm);
+  a.ps = reinterpret_cast<float *>(d.base + w.ps);
+  a.cnt_top = d.cnt_top;
+  a.ws_hdr = d.hdr;
+  a.ws_pairs = (int)pairs;
+  a.ws_room = (int)(((size_t)(reinterpret_cast<char *>(d.cnt_top) - d.base) - w.parts) / kLine);
+  a.P = w.P;
+}
 
 // A caller's workspace: header in the last line below the rounded-down end,
 // counters below it.
@@ -315,7 +329,6 @@ int decode_attention_ws(const void *q, int q_dtype, const uint8_t *k_indices, co
                      w.parts, pairs, wsd->part_bytes, wsd->pairs);
   }
   AttnArgs a = base_args();
-  char *ws = wsd->base;
   a.q = q;
   a.q_dtype = q_dtype;
   a.k_idx = k_indices;
@@ -330,14 +343,7 @@ int decode_attention_ws(const void *q, int q_dtype, const uint8_t *k_indices, co
   a.kv_head_stride = kv_head_stride;
   a.seq_stride = seq_stride;
   a.softmax_scale = softmax_scale;
-  a.po = reinterpret_cast<float *>(ws + w.po);
-  a.pm = reinterpret_cast<float *>(ws + w.pm);
-  a.ps = reinterpret_cast<float *>(ws + w.ps);
-  a.cnt_top = wsd->cnt_top;
-  a.ws_hdr = wsd->hdr;
-  a.ws_pairs = (int)pairs;
-  a.ws_room = (int)(((size_t)(reinterpret_cast<char *>(wsd->cnt_top) - ws) - w.parts) / kLine);
-  a.P = w.P;
+  set_workspace(a, w, *wsd, pairs);
   a.out = out;
   a.out_dtype = out_dtype;
   a.rq = rq;
@@ -397,6 +403,80 @@ extern "C" int tq_tq_decode_attention(const void *q, int q_dtype, const uint8_t 
                                kv_lens, max_kv_len, batch, num_heads, num_kv_heads, head_dim, bits, 0, norm_mode,
                                max_kv_len, kv_head_stride, seq_stride, softmax_scale, out, out_dtype, workspace,
                                workspace_bytes, stream, qjl_sign_matrix);
+}
+
+extern "C" int tq_paged_decode_attention(const void *q, int q_dtype, const uint8_t *k_indices,
+                                         const uint16_t *k_scales, const uint8_t *v_indices, const uint16_t *v_scales,
+                                         const uint8_t *signs, const uint16_t *norms, const uint32_t *sign_matrix,
+                                         const int *block_table, int table_width, const int *kv_lens, int batch,
+                                         int num_heads, int num_kv_heads, int head_dim, int bits,
+                                         size_t outlier_blocks, int norm_mode, int page_size, long long num_pages,
+                                         int max_kv_len, float softmax_scale, void *out, int out_dtype,
+                                         void *workspace, size_t workspace_bytes, hipStream_t stream) {
+  PageArgs pages{};
+  tqh::PolarCodec codec;
+  int rc = tqh::check_pages(num_pages, num_kv_heads, page_size, head_dim, bits, outlier_blocks, norm_mode, pages.shift,
+                            codec);
+  if (rc) return rc;
+  rc = check_common(num_heads, num_kv_heads, head_dim, bits, 0);
+  if (rc) return rc;
+  const int mode = codec.outlier ? kModePqo : (signs ? kModeTq : kModePq);
+  if (signs && codec.outlier)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "QJL correction applies to the standard codebook (outlier_blocks 0)");
+  if (signs && head_dim == 32)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "the QJL-corrected decode takes head_dim 64, 128 or 256");
+  if (!tqh::valid_dtype(q_dtype) || !tqh::valid_dtype(out_dtype))
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "unknown dtype");
+  if (batch < 0 || batch > 65535) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "batch %d outside 0 to 65,535", batch);
+  if (table_width < 0 || max_kv_len < 0 || max_kv_len > (long long)table_width << pages.shift)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "max_kv_len %d exceeds a table row of %d pages", max_kv_len, table_width);
+  if (max_kv_len > 1 << 27)  // the merge addresses a round's partials with 32-bit offsets
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "max_kv_len %d exceeds 2^27", max_kv_len);
+  if (batch == 0) return TQ_OK;
+  if (!q || !out || !kv_lens || !k_indices || !k_scales || !v_indices || !v_scales || (max_kv_len && !block_table) ||
+      (signs && (!norms || !sign_matrix)) || !workspace)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "null pointer");
+  for (const void *p : {(const void *)k_indices, (const void *)v_indices, (const void *)k_scales, (const void *)v_scales})
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+      return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "code and scale pools start on 16-byte boundaries");
+  const WsLayout w = ws_layout(batch, num_heads, num_kv_heads, head_dim, max_kv_len);
+  if (workspace_bytes < w.total)
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "workspace too small: %zu < %zu", workspace_bytes, w.total);
+  if (max_kv_len == 0 || num_pages == 0) return zero_output(out, (long long)batch * num_heads * head_dim, out_dtype, stream);
+  AttnArgs a = base_args();
+  a.q = q;
+  a.q_dtype = q_dtype;
+  a.k_idx = k_indices;
+  a.k_sc = k_scales;
+  a.v_idx = v_indices;
+  a.v_sc = v_scales;
+  a.kv_lens = kv_lens;
+  a.max_len = max_kv_len;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.softmax_scale = softmax_scale;
+  const DecodeWs d = caller_ws(workspace, workspace_bytes);
+  set_workspace(a, w, d, (long long)batch * num_kv_heads);
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.rmat = sign_matrix;
+  a.qjl_inv = tqh::inv_sqrt_dim(head_dim);
+  a.qjl_signs = reinterpret_cast<const uint32_t *>(signs);
+  a.qjl_norms = norms;
+  a.qjl_c = tq_qjl_bias_scale(head_dim);
+  // The passes that contract 4-bit codes before their offset is taken off lose
+  // up to 1e-3 of a long context's small outputs: a bf16 result's own rounding
+  // is larger, f16 and f32 results take the codebook.
+  if (codec.norm_mode == TQ_NORM_L2NORM || out_dtype != TQ_DTYPE_BF16) {
+    a.cb_args = 1;
+    for (int i = 0; i < codec.cb.nc; i++) a.cb[i] = codec.cb.c[i];
+  }
+  a.nr = num_heads / num_kv_heads;
+  pages.table = block_table;
+  pages.width = table_width;
+  pages.num_pages = (int)num_pages;
+  return launch_stream<true>(a, bits, mode, head_dim, dim3((unsigned)w.P, (unsigned)num_kv_heads, (unsigned)batch),
+                             stream, &pages);
 }
 
 extern "C" int tq_pqo_decode_attention(const void *q, int q_dtype, const uint8_t *k_indices, const uint16_t *k_scales,

@@ -6,6 +6,6 @@
 #include "tq_decode_kernel.h"
 
 namespace tqa {
-template void launch_stream_bm<4, kModeTq, true>(AttnArgs &, int, int, dim3, hipStream_t, tqh::AppendToken *);
-template void launch_stream_bm<4, kModeTq, false>(AttnArgs &, int, int, dim3, hipStream_t, tqh::AppendToken *);
+template void launch_stream_bm<4, kModeTq, true, tqh::AppendToken>(AttnArgs &, int, int, dim3, hipStream_t, tqh::AppendToken *);
+template void launch_stream_bm<4, kModeTq, false, tqh::AppendToken>(AttnArgs &, int, int, dim3, hipStream_t, tqh::AppendToken *);
 }  // namespace tqa

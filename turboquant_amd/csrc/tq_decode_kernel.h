@@ -261,7 +261,9 @@ __device__ __forceinline__ void store_new_token(const AppendArgs &ap, const uint
 // instance of its own, so that the launches given rq carry none of its code
 // APPEND: the launch stores one new token of every KV head first, in the
 // workgroup that holds the sequence's last token (the only one that reads it)
-template <class C, bool INLINE_MERGE, bool GRID, bool MULTI, bool PROJ = false, bool APPEND = false>
+// PAGED: the records lie in pages (PageArgs); k_idx .. v_sc are the pools and
+// the strides are not used
+template <class C, bool INLINE_MERGE, bool GRID, bool MULTI, bool PROJ = false, bool APPEND = false, bool PAGED = false>
 #ifndef TQ_DECODE_WPE
 #define TQ_DECODE_WPE 2
 #endif
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
                                                                const uint16_t *k_sc, const uint16_t *v_sc,
                                                                long long seq_stride, long long kv_head_stride,
                                                                int len_hint, AttnArgs a,
-                                                               std::conditional_t<APPEND, AppendArgs, NoAppend> ap) {
+                                                               std::conditional_t<PAGED, PageArgs, std::conditional_t<APPEND, AppendArgs, NoAppend>> ap) {
   constexpr int BITS = C::BITS, HD = C::HD, NQB = C::NQB, HG = C::HG, TPW = C::TPW, QW = C::QW, NW = C::NW;
   static_assert(GRID ? C::G_LDS_OK : C::LDS_OK, "the workgroup's LDS (with the merge's scratch) fits 160 KiB");
   // word offset of the layout from OFF_W on (the grid passes need no
@@ -331,54 +333,80 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   asm volatile("" ::"s"(a_q), "s"(a_sg), "s"(a_cb), "s"(a_rq), "s"(a_ws), "s"(a_lens), "s"(a_qdt), "s"(a_ngroups),
                "s"(a_nr), "s"(a_heads), "s"(a_max), "s"(a_cpr));
   // ---- balanced split (range launches with a.bal_nwg > 0, one head group
-  // per KV head, at most 64 sequences): the ranges' length S (in chunks) is
+  // per KV head, at most kBalSeqs sequences): the ranges' length S (in chunks) is
   // the smallest whose ranges, sequence b's chunks split into
   // R_b = ceil(n_b / S) near-equal ranges per KV head, number at most
   // bal_nwg.  Ragged batches then give every workgroup at most S chunks;
   // ranges of one fixed length would leave the compute units that hold the
   // long sequences' ranges setting the time.  A wave holds the batch's chunk
-  // counts (one sequence per lane), so the split costs a few reductions and
+  // counts (one sequence per lane; over pages up to four), so the split costs a few reductions and
   // a ballot, no LDS and no barrier before the first loads. ----
   int bal_ck0 = 0, bal_nck = 0, bal_nparts = 0;
   const bool bal = MULTI && a.bal_nwg > 0;
   if constexpr (MULTI) {
     if (bal) {
       const int nwg = a.bal_nwg, ny = a.bal_ny, nb = a.bal_batch;
-      int n = 0;
-      if (lane < nb) {
-        const int lb = len_hint >= 0 ? len_hint : min(max(a_lens[lane], 0), a_max);
-        n = (lb + C::CHUNK - 1) / C::CHUNK;
+      constexpr int SQ = kBalSeqs<PAGED> / 64;  // sequences a lane holds: lane, 64 + lane, ..
+      int n[SQ], T = 0, most = 0;
+#pragma unroll
+      for (int k = 0; k < SQ; k++) {
+        n[k] = 0;
+        if (64 * k + lane < nb) {
+          const int lb = len_hint >= 0 ? len_hint : min(max(a_lens[64 * k + lane], 0), a_max);
+          n[k] = (lb + C::CHUNK - 1) / C::CHUNK;
+        }
+        T += wave_sum_i(n[k]);
+        most = max(most, wave_max_i(n[k]));
       }
       // S: the closed form ceil(ny T / (nwg - ny nb)) (feasible: sum_b
       // ceil(n_b / S) <= T / S + nb), or one less when that still fits
-      const int T = wave_sum_i(n);
-      int S = nwg > ny * nb ? (int)(((long long)T * ny + (nwg - ny * nb) - 1) / (nwg - ny * nb)) : wave_max_i(n);
+      int S = nwg > ny * nb ? (int)(((long long)T * ny + (nwg - ny * nb) - 1) / (nwg - ny * nb)) : most;
       S = max(S, 1);
-      if (S > 1 && (long long)wave_sum_i((n + S - 2) / (S - 1)) * ny <= nwg) S--;
+      if (S > 1) {
+        int less = 0;
+#pragma unroll
+        for (int k = 0; k < SQ; k++) less += wave_sum_i((n[k] + S - 2) / (S - 1));
+        if ((long long)less * ny <= nwg) S--;
+      }
       S = __builtin_amdgcn_readfirstlane(S);
-      const int rb = (n + S - 1) / S;  // ranges per KV head of the lane's sequence
-      const int incl = wave_incl_scan_i(rb);
-      const int pre = incl - rb;  // ranges before the lane's sequence, per KV head
+      int rb[SQ], pre[SQ], ranges = 0;  // ranges per KV head of the lane's sequences, and before each
+#pragma unroll
+      for (int k = 0; k < SQ; k++) {
+        rb[k] = (n[k] + S - 1) / S;
+        const int incl = wave_incl_scan_i(rb[k]);
+        pre[k] = ranges + incl - rb[k];
+        ranges += __builtin_amdgcn_readlane(incl, 63);
+      }
       const int wi = blockIdx.x;
-      const int total = __builtin_amdgcn_readlane(incl, 63) * ny;
+      const int total = ranges * ny;
       // empty sequences attend to nothing: zero output (cuda/attention.rs:65-68)
-      for (int bb = wi; bb < nb; bb += nwg)
-        if (__builtin_amdgcn_readlane(n, bb) == 0)
-          for (int e = tid; e < a_heads * HD; e += C::THREADS) {
-            const long long oi = (long long)bb * a_heads * HD + e;
-            if (a.out_dtype == kF32) static_cast<float *>(a.out)[oi] = 0.f;
-            else static_cast<uint16_t *>(a.out)[oi] = 0;
-          }
+#pragma unroll
+      for (int k = 0; k < SQ; k++)
+        for (int bb = 64 * k + wi; bb < min(nb, 64 * k + 64); bb += nwg)
+          if (__builtin_amdgcn_readlane(n[k], bb - 64 * k) == 0)
+            for (int e = tid; e < a_heads * HD; e += C::THREADS) {
+              const long long oi = (long long)bb * a_heads * HD + e;
+              if (a.out_dtype == kF32) static_cast<float *>(a.out)[oi] = 0.f;
+              else static_cast<uint16_t *>(a.out)[oi] = 0;
+            }
       if (wi >= total) {
         __builtin_amdgcn_s_waitcnt(0);
         return;
       }
       // workgroup wi: sequence b (the last whose ranges start at or before
       // it), KV head y, range r of its R_b
-      const unsigned long long le = __ballot(lane < nb && pre * ny <= wi);
-      b = __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(le));
-      const int pre_b = __builtin_amdgcn_readlane(pre, b), r_b = __builtin_amdgcn_readlane(rb, b);
-      const int n_b = __builtin_amdgcn_readlane(n, b);
+      int pre_b = 0, r_b = 1, n_b = 0;
+#pragma unroll
+      for (int k = 0; k < SQ; k++) {
+        const unsigned long long le = __ballot(64 * k + lane < nb && pre[k] * ny <= wi);
+        if (le) {
+          const int l = __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(le));
+          b = 64 * k + l;
+          pre_b = __builtin_amdgcn_readlane(pre[k], l);
+          r_b = __builtin_amdgcn_readlane(rb[k], l);
+          n_b = __builtin_amdgcn_readlane(n[k], l);
+        }
+      }
       const int k = wi - pre_b * ny;
       y = k / r_b;
       const int r = k - y * r_b;
@@ -482,7 +510,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   // Buffer loads bounded by the sequence's len records: a token past the end
   // reads zeros (its score is masked and its weight is 0), and a tile's
   // offset is a scalar constant. ----
-  const long long rec0 = (long long)b * seq_stride + (long long)g * kv_head_stride;
+  const long long rec0 = PAGED ? 0 : (long long)b * seq_stride + (long long)g * kv_head_stride;
   const uint32_t nrec = (uint32_t)len;
   const uint8_t *kbase = k_idx + rec0 * PACKED, *vbase = v_idx + rec0 * PACKED;
   const uint16_t *ksbase = k_sc + rec0 * NQB, *vsbase = v_sc + rec0 * NQB;
@@ -499,6 +527,39 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   uint32_t sgw[NKT][C::SW4];
   uint32_t nrm[NKT];
   uint32_t vsr[C::TPL][(NQB + 1) / 2];
+  // Pages: a tile's 16 tokens lie in one (page sizes are multiples of 16), so
+  // a wave holds one page per tile, uniform, and a lane the page of its V-scale
+  // tokens, from one gather of table entries a chunk (the next chunk's goes out
+  // with this chunk's first tiles).  A tile past the sequence's end or in an
+  // entry outside the pool has no records.
+  int vpage = -1, vpage_next = -1;
+  int pages[PAGED ? NKT : 1];
+  auto gather_pages = [&](uint32_t tw0) -> int {
+    if constexpr (PAGED) {
+      const int t = (int)tw0 + C::TPL * lane;
+      return t < len ? ap.table[(long long)b * ap.width + (t >> ap.shift)] : -1;
+    } else {
+      return -1;
+    }
+  };
+  auto take_pages = [&](int v) {
+    if constexpr (PAGED) {
+      vpage = (uint32_t)v < (uint32_t)ap.num_pages ? v : -1;
+#pragma unroll
+      for (int i = 0; i < NKT; i++) pages[i] = __builtin_amdgcn_readlane(vpage, 16 * i / C::TPL);
+    }
+  };
+  // tile i of the wave's tokens from tw0 on: its first record and how many
+  // of its 16 there are
+  auto tile_rec = [&](int i, uint32_t t16) -> long long {
+    if constexpr (PAGED)
+      return (((long long)max(pages[i], 0) * a.num_kv_heads + g) << ap.shift) + (t16 & ((1u << ap.shift) - 1u));
+    else return 0;
+  };
+  auto tile_count = [&](int i, uint32_t t16) -> int {
+    if constexpr (PAGED) return pages[i] < 0 ? 0 : min(max(len - (int)t16, 0), 16);
+    else return 0;
+  };
   // The wave's loads form one stream of groups, consumed in order: K tile i
   // (records, scales, QJL signs and norms) is group i, the V scales group
   // NKT, V tile i group NKT + 1 + i.  Only a few groups are in flight at a
@@ -508,17 +569,20 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     if (grp < NKT) {
       const int i = grp;
       const uint32_t t16 = tw0 + 16u * i;  // the tile's first token
-      const auto rk = rec_rsrc(kbase, nrec * PACKED, t16 * PACKED);
-      const auto rks = rec_rsrc(ksbase, nrec * NQB * 2u, t16 * NQB * 2u);
+      const long long trec = tile_rec(i, t16);
+      const uint32_t tn = (uint32_t)tile_count(i, t16);
+      const auto rk = PAGED ? rec_rsrc(k_idx + trec * PACKED, tn * PACKED) : rec_rsrc(kbase, nrec * PACKED, t16 * PACKED);
+      const auto rks = PAGED ? rec_rsrc(k_sc + trec * NQB, tn * NQB * 2u) : rec_rsrc(ksbase, nrec * NQB * 2u, t16 * NQB * 2u);
 #pragma unroll
       for (int qg = 0; qg < QG; qg++) {
         buf_words<NW>(kw[i][qg], rk, kvo + qg * QPM * QW * 4, 0);
         ksv[i][qg] = __builtin_amdgcn_raw_buffer_load_b16(rks, kso + qg * QPM * 2, 0, 0);
       }
       if constexpr (C::QJL) {
-        const auto rsg = rec_rsrc(reinterpret_cast<const uint8_t *>(a.qjl_signs) + rec0 * (HD / 8), nrec * (HD / 8),
-                                  t16 * (HD / 8));
-        const auto rnm = rec_rsrc(a.qjl_norms + rec0, nrec * 2u, t16 * 2u);
+        const uint8_t *const sgb = reinterpret_cast<const uint8_t *>(a.qjl_signs);
+        const auto rsg = PAGED ? rec_rsrc(sgb + trec * (HD / 8), tn * (HD / 8))
+                               : rec_rsrc(sgb + rec0 * (HD / 8), nrec * (HD / 8), t16 * (HD / 8));
+        const auto rnm = PAGED ? rec_rsrc(a.qjl_norms + trec, tn * 2u) : rec_rsrc(a.qjl_norms + rec0, nrec * 2u, t16 * 2u);
 #pragma unroll
         for (int s4 = 0; s4 < C::SW4; s4++) {
           const int wi = min(s4 * 4 + lg, NQB - 1);
@@ -528,6 +592,38 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
       }
     } else if (grp == NKT) {
       // V scales of the wave: tokens tw + TPL lane + u, all NQB per token
+      if constexpr (PAGED) {
+        // a lane's tokens lie in one page; a page past 4 GiB of scales is
+        // out of a descriptor's reach, so the address is the lane's own.  The
+        // token behind the last one is in the page, and masked at its use.
+#pragma unroll
+        for (int u = 0; u < C::TPL; u++)
+#pragma unroll
+          for (int j = 0; j < (NQB + 1) / 2; j++) vsr[u][j] = 0u;
+        const int t = (int)tw0 + C::TPL * lane;
+        if (vpage >= 0 && t < len) {
+          const uint16_t *p = v_sc + ((((long long)vpage * a.num_kv_heads + g) << ap.shift) + (t & ((1 << ap.shift) - 1))) * NQB;
+#pragma unroll
+          for (int u = 0; u < C::TPL; u++) {
+            if constexpr (NQB == 1) {
+              vsr[u][0] = p[u];
+            } else if constexpr (NQB == 2) {
+              vsr[u][0] = reinterpret_cast<const uint32_t *>(p)[u];
+            } else if constexpr (NQB == 4) {
+              const uint2 v = reinterpret_cast<const uint2 *>(p)[u];
+              vsr[u][0] = v.x;
+              vsr[u][1] = v.y;
+            } else {
+              const uint4 v = reinterpret_cast<const uint4 *>(p)[u];
+              vsr[u][0] = v.x;
+              vsr[u][1] = v.y;
+              vsr[u][2] = v.z;
+              vsr[u][3] = v.w;
+            }
+          }
+        }
+        return;
+      }
       const auto rvs = rec_rsrc(vsbase, nrec * NQB * 2u, tw0 * NQB * 2u);
       const uint32_t vso = (uint32_t)(C::TPL * lane) * NQB * 2u;
 #pragma unroll
@@ -537,7 +633,9 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
       }
     } else {
       const int i = grp - NKT - 1;
-      const auto rv = rec_rsrc(vbase, nrec * PACKED, (tw0 + 16u * i) * PACKED);
+      const uint32_t t16 = tw0 + 16u * i;
+      const auto rv = PAGED ? rec_rsrc(v_idx + tile_rec(i, t16) * PACKED, (uint32_t)tile_count(i, t16) * PACKED)
+                            : rec_rsrc(vbase, nrec * PACKED, t16 * PACKED);
       if constexpr (GRID) {
         load_words<NQB>(vg[i], rv, (uint32_t)lane * (4u * NQB));
       } else {
@@ -577,6 +675,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     late = (len - 1) / C::CHUNK == ck0;
     if (late) store_new_token<C>(ap, rsw, a.qjl_inv, g, rec0 + len - 1, tid, lane, wave);
   }
+  if constexpr (PAGED) take_pages(gather_pages(tw_first));
   if (!late) issue_first(tw_first, LA0);
   auto issue_k = [&](int i, uint32_t tw0) {  // K tile i is being consumed
     if (i == 0) {
@@ -888,6 +987,9 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   for (int ck = 0; ck < nck; ck++) {
   const int tw = (ck0 + ck) * C::CHUNK + wave * TPW;
   const uint32_t tw0 = (uint32_t)tw;
+  if constexpr (PAGED && MULTI) {
+    if (ck + 1 < nck) vpage_next = gather_pages(tw0 + C::CHUNK);
+  }
   // range launches: the K pass above the softmax in wave priority, the V
   // pass above both (C4 56.7 -> 55.5 us; single-chunk launches measured
   // no gain from the K-pass step)
@@ -972,7 +1074,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
       y[0] = x[0] + x[1];
       if constexpr (QPM == 4) y[0] = sum_xor16(y[0]);
     }
-    const bool tok_ok = tw + 16 * i + l16 < len;
+    const bool tok_ok = PAGED ? l16 < tile_count(i, tw0 + 16u * i) : tw + 16 * i + l16 < len;
 #pragma unroll
     for (int v = 0; v < NS; v++) {
       float s = y[v] * escale[v];
@@ -1018,6 +1120,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     for (int qb = 0; qb < NQB; qb++) {
       const uint32_t bits = NQB == 1 ? vsr[u][0] : (vsr[u][qb >> 1] >> (16 * (qb & 1)));
       svv[u][qb] = fabsf(f16_to_f32((uint16_t)(bits & 0xffffu)));
+      if (PAGED && u > 0 && tw + C::TPL * lane + u >= len) svv[u][qb] = 0.f;  // what lies behind the last token
       smax = fmaxf(smax, svv[u][qb]);
     }
   // the running exponent Ev is the largest of the range's chunks so far; the
@@ -1075,7 +1178,10 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
       for (int u = 4; u < 8; u++)
         if (4 * bk + u < NKT) issue(NKT + 1 + 4 * bk + u, tw0);
     }
-    if (MULTI && bk == NB - 1 && ck + 1 < nck) issue_first(tw0 + C::CHUNK, LA);
+    if (MULTI && bk == NB - 1 && ck + 1 < nck) {
+      take_pages(vpage_next);  // this chunk's tiles have all gone out
+      issue_first(tw0 + C::CHUNK, LA);
+    }
     // stage the block's four tiles: lane l holds token l / 4 of its tile,
     // bytes 4 NQB (l % 4) .. of the record
 #pragma unroll
@@ -1168,7 +1274,10 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
 #pragma unroll
   for (int vp = 0; vp < NVP; vp++) {
     issue_v(vp, tw0);
-    if (MULTI && vp == VP_NEXT && ck + 1 < nck) issue_first(tw0 + C::CHUNK, LA);
+    if (MULTI && vp == VP_NEXT && ck + 1 < nck) {
+      take_pages(vpage_next);  // this chunk's tiles have all gone out
+      issue_first(tw0 + C::CHUNK, LA);
+    }
     u32x4 bw[QG];
 #pragma unroll
     for (int vs = 0; vs < QG; vs++) {
@@ -1367,10 +1476,13 @@ int resident_workgroups() {
 }
 
 // 4-bit codes on the compiled-in MaxNorm codebook (evenly spaced) take the
-// grid key pass; a caller's codebook or the L2Norm tables, the pair table
-template <class C, bool INLINE, bool MULTI>
-void launch_stream_k(AttnArgs &a, dim3 grid, hipStream_t st, int len_hint, tqh::AppendToken *ap) {
-  if constexpr (INLINE && !MULTI) {
+// grid key pass; a caller's codebook or the L2Norm tables, the pair table.
+// X: what a launch does beside attending: AppendToken (null: nothing), or
+// PageArgs for records in pages.
+template <class C, bool INLINE, bool MULTI, class X>
+void launch_stream_k(AttnArgs &a, dim3 grid, hipStream_t st, int len_hint, X *ap) {
+  constexpr bool PAGED = std::is_same_v<X, PageArgs>;
+  if constexpr (INLINE && !MULTI && !PAGED) {
     if (ap) {
       AppendArgs x{};
       x.k = ap->k;
@@ -1395,9 +1507,11 @@ void launch_stream_k(AttnArgs &a, dim3 grid, hipStream_t st, int len_hint, tqh::
       return;
     }
   }
-  if (ap) {  // range launches: long contexts, where a launch more does not show
-    ap->rc = store_token_apart(*ap, a, st);
-    if (ap->rc) return;
+  if constexpr (!PAGED) {
+    if (ap) {  // range launches: long contexts, where a launch more does not show
+      ap->rc = store_token_apart(*ap, a, st);
+      if (ap->rc) return;
+    }
   }
   auto go = [&](auto k) {
     constexpr auto kernel = decltype(k)::value;
@@ -1409,19 +1523,23 @@ void launch_stream_k(AttnArgs &a, dim3 grid, hipStream_t st, int len_hint, tqh::
                            max((long long)resident_workgroups<kernel, C::THREADS>() * device_cus(), pairs));
       grid = dim3((unsigned)a.bal_nwg, 1u, 1u);
     }
-    hipLaunchKernelGGL(kernel, grid, dim3(C::THREADS), 0, st, a.k_idx, a.v_idx, a.k_sc, a.v_sc, a.seq_stride,
-                       a.kv_head_stride, len_hint, a, NoAppend{});
+    if constexpr (PAGED)
+      hipLaunchKernelGGL(kernel, grid, dim3(C::THREADS), 0, st, a.k_idx, a.v_idx, a.k_sc, a.v_sc, 0ll, 0ll, len_hint, a,
+                         *ap);
+    else
+      hipLaunchKernelGGL(kernel, grid, dim3(C::THREADS), 0, st, a.k_idx, a.v_idx, a.k_sc, a.v_sc, a.seq_stride,
+                         a.kv_head_stride, len_hint, a, NoAppend{});
   };
   if constexpr (C::BITS == 4 && C::MODE == kModePqo) {
-    if (!a.cb_dev && !a.cb_args) return go(Kernel<stream_decode_kernel<C, INLINE, true, MULTI>>{});
+    if (!a.cb_dev && !a.cb_args) return go(Kernel<stream_decode_kernel<C, INLINE, true, MULTI, false, false, PAGED>>{});
   }
-  if constexpr (C::QJL) {
-    if (!a.rq) return go(Kernel<stream_decode_kernel<C, INLINE, false, MULTI, true>>{});
+  if constexpr (C::QJL) {  // over pages the launch always projects the query
+    if (PAGED || !a.rq) return go(Kernel<stream_decode_kernel<C, INLINE, false, MULTI, true, false, PAGED>>{});
   }
-  go(Kernel<stream_decode_kernel<C, INLINE, false, MULTI>>{});
+  if constexpr (!C::QJL || !PAGED) go(Kernel<stream_decode_kernel<C, INLINE, false, MULTI, false, false, PAGED>>{});
 }
-template <class C, bool INLINE>
-void launch_stream_c(AttnArgs &a, dim3 grid, hipStream_t st, tqh::AppendToken *ap) {
+template <class C, bool INLINE, class X>
+void launch_stream_c(AttnArgs &a, dim3 grid, hipStream_t st, X *ap) {
   a.chunk = C::CHUNK;
   const int chunks = (a.max_len + C::CHUNK - 1) / C::CHUNK;
   // Chunks per workgroup: one while the grid of single chunks fits one round
@@ -1446,12 +1564,12 @@ void launch_stream_c(AttnArgs &a, dim3 grid, hipStream_t st, tqh::AppendToken *a
       a.cpr = (int)min((long long)max(chunks, 1), (tasks + TQ_RANGE_WGS * cus - 1) / (TQ_RANGE_WGS * cus));
       // Balanced split: as many near-equal ranges as the compute units hold
       // at once (up to TQ_BAL_WGS per unit), for one head group per KV head
-      // and at most 64 sequences (a wave holds their chunk counts).  Ragged
+      // and at most kBalSeqs sequences (a wave holds their chunk counts).  Ragged
       // batches then load every compute unit alike; with ranges of a fixed
       // length, a unit that holds two full ranges of long sequences sets the
       // time.  Measured at C4: 64.3 -> 58.6 us; 16 sequences all at 16,384
       // tokens 66.6 -> 67.2 us.
-      if (TQ_BALANCE && a.ngroups == 1 && grid.z <= 64u) {
+      if (TQ_BALANCE && a.ngroups == 1 && grid.z <= (unsigned)kBalSeqs<std::is_same_v<X, PageArgs>>) {
         a.bal_nwg = (int)-min(tasks, (long long)1 << 30);  // negative: sized by launch_stream_k
         a.bal_batch = (int)grid.z;
         a.bal_ny = (int)grid.y;
@@ -1479,8 +1597,8 @@ void launch_stream_c(AttnArgs &a, dim3 grid, hipStream_t st, tqh::AppendToken *a
 // the halved split-K merge is on the critical path), else 4 waves (several
 // workgroups per compute unit keep more waves per SIMD in flight).  The
 // reference ABI (a separate merge launch) always takes the 8-wave form.
-template <int BITS, int MODE, int NQB, int HG, bool INLINE>
-void launch_stream_cfg(AttnArgs &a, dim3 grid, hipStream_t st, tqh::AppendToken *ap) {
+template <int BITS, int MODE, int NQB, int HG, bool INLINE, class X>
+void launch_stream_cfg(AttnArgs &a, dim3 grid, hipStream_t st, X *ap) {
   using C = StreamCfg<BITS, MODE, NQB, HG>;
   using C4 = StreamCfg4<BITS, MODE, NQB, HG>;
   using C64 = StreamCfg64<BITS, MODE, NQB, HG>;
@@ -1514,14 +1632,14 @@ void launch_stream_cfg(AttnArgs &a, dim3 grid, hipStream_t st, tqh::AppendToken 
   }
   launch_stream_c<C, INLINE>(a, grid, st, ap);
 }
-template <int BITS, int MODE, int NQB, bool INLINE>
-void launch_stream_hg(AttnArgs &a, int hg, dim3 grid, hipStream_t st, tqh::AppendToken *ap) {
+template <int BITS, int MODE, int NQB, bool INLINE, class X>
+void launch_stream_hg(AttnArgs &a, int hg, dim3 grid, hipStream_t st, X *ap) {
   if (hg == 2) launch_stream_cfg<BITS, MODE, NQB, 2, INLINE>(a, grid, st, ap);
   else if (hg == 4) launch_stream_cfg<BITS, MODE, NQB, 4, INLINE>(a, grid, st, ap);
   else launch_stream_cfg<BITS, MODE, NQB, 8, INLINE>(a, grid, st, ap);
 }
-template <int BITS, int MODE, bool INLINE>
-void launch_stream_nqb(AttnArgs &a, int nqb, int hg, dim3 grid, hipStream_t st, tqh::AppendToken *ap) {
+template <int BITS, int MODE, bool INLINE, class X>
+void launch_stream_nqb(AttnArgs &a, int nqb, int hg, dim3 grid, hipStream_t st, X *ap) {
   if constexpr (MODE != kModeTq) {
     if (nqb == 1) return launch_stream_hg<BITS, MODE, 1, INLINE>(a, hg, grid, st, ap);
   }
@@ -1531,8 +1649,8 @@ void launch_stream_nqb(AttnArgs &a, int nqb, int hg, dim3 grid, hipStream_t st, 
 }
 }  // namespace
 
-template <int BITS, int MODE, bool INLINE>
-void launch_stream_bm(AttnArgs &a, int nqb, int hg, dim3 grid, hipStream_t st, tqh::AppendToken *ap) {
+template <int BITS, int MODE, bool INLINE, class X>
+void launch_stream_bm(AttnArgs &a, int nqb, int hg, dim3 grid, hipStream_t st, X *ap) {
   launch_stream_nqb<BITS, MODE, INLINE>(a, nqb, hg, grid, st, ap);
 }
 
