@@ -248,6 +248,34 @@ def test_rope_zeros_infinities_and_nan(tq):
     assert qo[1, 0].isnan().any() and qo[2, 1].isnan().all()
 
 
+def test_wrappers_refuse(tq):
+    """Shapes, types, strides and places that the wrappers check themselves."""
+    q, k, pos, f = torch.zeros(3, 4, 64).cuda(), torch.zeros(3, 2, 64).cuda(), i32(0, 1, 2), torch.ones(32).cuda()
+    layer = tq.PagedLayer.empty(2, 16, 2, 64, 3)
+    slots, ws = torch.arange(3).cuda(), tq.AttentionWorkspace(3, 4, 2, 64, 32)
+    table = torch.zeros((3, 2), dtype=torch.int32, device="cuda")
+    for call in (lambda: tq.qk_norm_rope(q, k, pos, f, out=(k, k)), lambda: tq.qk_norm_rope(q, k, pos.long(), f),
+                 lambda: tq.qk_norm_rope(q, k, pos, f.double()), lambda: tq.qk_norm_rope(q, k, pos, f, q[0, 0, :32]),
+                 lambda: tq.qk_norm_rope(q, k, pos, f, q[0, 0].half()), lambda: tq.qk_norm_rope(q, k, pos[:2], f),
+                 lambda: tq.qk_norm_rope(q, k, pos.cpu(), f), lambda: tq.qk_norm_rope(q.transpose(0, 1), k, pos, f),
+                 lambda: tq.paged_store(layer, slots, k, k, 4), lambda: tq.paged_store(layer, slots, k, k.half(), 3),
+                 lambda: tq.paged_store(layer, slots.int(), k, k, 3), lambda: tq.paged_store(layer, slots, q, q, 3),
+                 lambda: tq.paged_store(layer, slots, k, k, 3, 0, sign_matrix=f),
+                 lambda: tq.paged_load(layer, slots, 3, out=(k, k.half())),
+                 lambda: tq.paged_load(layer, slots[::2], 3, out=(k[:2], k[:2])),
+                 lambda: tq.paged_decode_attention(q[:, :, :32], layer, table, pos, 3, 32, 1.0, ws),
+                 lambda: tq.paged_decode_attention(q, layer, table, pos.long(), 3, 32, 1.0, ws),
+                 lambda: tq.paged_decode_attention(q, layer, table[:2], pos, 3, 32, 1.0, ws),
+                 lambda: tq.paged_decode_attention(q, layer, table, pos, 3, 32, 1.0, ws, sign_matrix=f.int()),
+                 lambda: tq.paged_plan(pos, pos, table, pos[::2], pos[:1], 16, 3),
+                 lambda: tq.paged_plan(pos, pos[:2], table, pos, pos[:1], 16, 3),
+                 lambda: tq.paged_plan(pos, pos, table, pos, pos[:1], 16, -1)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(tq.TurboQuantError, match="exceeds a table row"):
+        tq.paged_decode_attention(q, layer, table, pos, 3, 33, 1.0, ws)
+
+
 # ---------------------------------------------------------------- records in pages
 
 def layer_and_slots(tq, rng, t, page, hk, d, bits, qjl, spare=2):

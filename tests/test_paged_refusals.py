@@ -140,8 +140,6 @@ def test_rope_wrapper_shapes():
         tq.qk_norm_rope(q, k.half(), pos, f)
     with pytest.raises(ValueError, match="one type"):
         tq.qk_norm_rope(q, k[:2], pos, f)
-    with pytest.raises(ValueError, match="shapes and type"):
-        tq.qk_norm_rope(q, k, pos, f, out=(k, k))
 
 
 def test_cache_arguments():

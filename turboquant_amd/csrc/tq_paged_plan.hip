@@ -17,6 +17,10 @@ using namespace tqm;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kMaxTokens = 1 << 24, kMaxWidth = 1 << 20;
+#ifndef TQ_PLAN_APART
+#define TQ_PLAN_APART 4096
+#endif
+constexpr int kApart = TQ_PLAN_APART;  // steps of more tokens: their rows by a launch of their own
 // A request with at most this many new pages and tokens is written by its own
 // lane, a larger one by a wave.
 constexpr int kLaneItems = 2;
@@ -28,6 +32,7 @@ struct PlanArgs {
   long long *slots;
   int *positions, *starts, *appended, *kv_out, *free_out;
   int batch, width, capacity, shift, tokens;
+  int apart;  // the tokens' rows are another launch's
 };
 
 // Exclusive prefix sum of v over the workgroup's threads, and their total.
@@ -130,30 +135,78 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
       a.appended[b] = fits ? n : 0;
       a.kv_out[b] = raw < 0 ? 0 : (fits ? kv + n : kv);
       const Item it{b, held, fits ? need : 0, kv, fits ? n : 0, (int)min(start, 0x7fffffffll), avail - 1 - taken};
-      if (fits && n <= kLaneItems) {
+      const int rows = a.apart ? 0 : n;
+      if (fits && rows <= kLaneItems && it.need <= kLaneItems) {
         for (int j = 0; j < it.need; j++) write_page(a, it, j);
-        for (int i = 0; i < n; i++) write_token(a, it, i);
-      } else if (n > 0 && start < a.tokens) {
+        for (int i = 0; i < rows; i++) write_token(a, it, i);
+      } else if (fits || (rows > 0 && start < a.tokens)) {
         s_item[atomicAdd(&s_items, 1)] = fits ? it : Item{b, -1, 0, 0, (int)min((long long)n, a.tokens - start), (int)start, 0};
       }
     }
     __syncthreads();
     const int items = s_items;
-    for (int k = wave; k < items; k += kWaves) {
-      const Item it = s_item[k];
-      if (it.held < 0) {  // it does not fit: its rows hold no tokens
-        for (int i = lane; i < it.n; i += 64) write_none(a, it.start + i);
-        continue;
+    for (int k = wave; k < items; k += 4 * kWaves) {
+      // four requests' first pages, their reads side by side
+      int page[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int ku = k + u * kWaves;
+        page[u] = ku < items && lane < s_item[ku].need ? a.free_pages[s_item[ku].top - lane] : 0;
       }
-      for (int j = lane; j < it.need; j += 64) write_page(a, it, j);
-      for (int i = lane; i < it.n; i += 64) write_token(a, it, i);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int ku = k + u * kWaves;
+        if (ku >= items) break;
+        const Item it = s_item[ku];
+        if (it.held < 0) {  // it does not fit: its rows hold no tokens
+          for (int i = lane; i < it.n; i += 64) write_none(a, it.start + i);
+          continue;
+        }
+        if (lane < it.need) a.table[(long long)it.b * a.width + it.held + lane] = page[u];
+        for (int j = 64 + lane; j < it.need; j += 64) write_page(a, it, j);
+        if (a.apart) continue;
+        for (int i = lane; i < it.n; i += 64) write_token(a, it, i);
+      }
     }
   }
   if (tid == 0) {
     a.starts[a.batch] = (int)min(start0, 0x7fffffffll);
     a.free_out[0] = (int)(avail - used);
   }
+  if (a.apart) return;
   for (long long t = start0 + tid; t < a.tokens; t += kThreads) write_none(a, (int)t);
+}
+
+// The rows of a step of many tokens, a lane a token: its request is the last
+// that starts at or before it (every kth start in LDS, then at most k more).
+constexpr int kStarts = 2048;
+__global__ __launch_bounds__(256) void paged_tokens_kernel(PlanArgs a, int k) {
+  __shared__ int s_start[kStarts];
+  const int n = (a.batch + k - 1) / k;  // <= kStarts
+  for (int i = threadIdx.x; i < n; i += 256) s_start[i] = a.starts[i * k];
+  __syncthreads();
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= a.tokens) return;
+  if (t >= a.starts[a.batch]) return write_none(a, t);
+  int lo = 0, hi = n;  // s_start[lo] <= t < s_start[hi]
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (s_start[m] <= t) lo = m;
+    else hi = m;
+  }
+  lo *= k;
+  hi = min(lo + k, a.batch);
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (a.starts[m] <= t) lo = m;
+    else hi = m;
+  }
+  const int got = a.appended[lo];
+  if (got == 0) return write_none(a, t);
+  const int pos = a.kv_out[lo] - got + (t - a.starts[lo]);
+  const int page = a.table[(long long)lo * a.width + (pos >> a.shift)];
+  a.slots[t] = page < 0 ? -1 : ((long long)page << a.shift) + (pos & ((1 << a.shift) - 1));
+  a.positions[t] = pos;
 }
 
 }  // namespace
@@ -177,7 +230,10 @@ extern "C" int tq_paged_plan(const int *kv_lens, const int *new_lens, int batch,
       (num_tokens && (!slots || !positions)))
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "null pointer");
   PlanArgs a{kv_lens, new_lens, block_table, free_pages, free_count, slots, positions, starts, appended, kv_lens_out,
-             free_count_out, batch, table_width, free_capacity, shift, num_tokens};
+             free_count_out, batch, table_width, free_capacity, shift, num_tokens, batch && num_tokens > kApart};
   hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+  if (a.apart)
+    hipLaunchKernelGGL(paged_tokens_kernel, dim3((unsigned)((num_tokens + 255) / 256)), dim3(256), 0, stream, a,
+                       (batch + kStarts - 1) / kStarts);
   return tqh::check_launch("paged_plan_kernel");
 }

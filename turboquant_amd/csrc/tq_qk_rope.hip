@@ -12,6 +12,7 @@
 #include "tq_mfma.h"
 #include "tq_paged.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -27,6 +28,7 @@ struct RopeArgs {
   const int *positions;
   const float *inv_freq;
   int tokens, head_dim, rot, half;
+  int splits;               // waves that share a token's rows
   float eps, inv_dim;
 };
 
@@ -119,67 +121,117 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// Where a rotated element's partner is: its neighbour in the lane; the same
+// element of lane ^ LPR / 2 (the whole row of 8 LPR elements turns); any
+// element of the row.
+enum Partner : int { kNeighbour = 0, kHalfRow = 1, kAny = 2 };
+
+constexpr int kWaves = 2048;  // waves that a launch of few tokens is split into
+constexpr int kBatch = 4;  // rows a lane has in flight
+
 // LPR lanes a row (a power of two, eight elements a lane; lanes past head_dim
-// hold zeros).  PAIRS: interleaved rotation.
-template <int LPR, int DT, bool VEC, bool PAIRS>
+// hold zeros).  A wave takes one token, or one of `splits` parts of its rows,
+// 64 / LPR rows a pass: the turns are formed once, a pair a lane, and kept as
+// each lane's eight through LDS.
+template <int LPR, int DT, bool VEC, int PARTNER>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
-  __shared__ __attribute__((aligned(16))) float s_row[PAIRS ? 1 : 256 * 8];
-  const int tid = threadIdx.x, l = tid % LPR, e0 = 8 * l;
-  const int rows = a.heads[0] + a.heads[1];
-  const long long row = (long long)blockIdx.x * (256 / LPR) + tid / LPR;
-  const long long t = row / rows;
-  const int h = (int)(row - t * rows);
+  constexpr int RPW = 64 / LPR, NT = PARTNER == kNeighbour ? 4 : 8;
+  __shared__ float2 s_turn[4][4 * LPR];
+  __shared__ __attribute__((aligned(16))) float s_row[PARTNER == kAny ? 4 : 1][PARTNER == kAny ? 512 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l = lane % LPR, e0 = 8 * l, r = lane / LPR;
+  const int id = blockIdx.x * 4 + wave;
+  const int t = id / a.splits, part = id - t * a.splits;
   if (t >= a.tokens) return;
-  const int which = h >= a.heads[0], hh = which ? h - a.heads[0] : h;
   const int pos = a.positions[t];
-  if (pos < 0) return;  // no token: whole rows of lanes leave
+  if (pos < 0) return;  // no token
   const bool in = e0 < a.head_dim;
-  float x[8] = {};
-  if (in) load8<DT, VEC>(a.x[which], t * a.in_stride[which] + (long long)hh * a.head_dim + e0, x);
-  if (a.weight[which]) {
-    float ss = 0.f;
+  const int passes_q = (a.heads[0] + RPW - 1) / RPW, passes = passes_q + (a.heads[1] + RPW - 1) / RPW;
+  const int p1 = (int)((long long)(part + 1) * passes / a.splits);
+  float x[kBatch][8];
+  auto head_of = [&](int p, int which) { return (which ? p - passes_q : p) * RPW + r; };
+  auto load = [&](int p0) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) ss = __builtin_fmaf(x[j], x[j], ss);
-    const float scale = 1.0f / sqrtf(__builtin_fmaf(row_sum<LPR>(ss), a.inv_dim, a.eps));
-    if (in) {
-      float w[8];
-      load8<DT, false>(a.weight[which], e0, w);
+    for (int u = 0; u < kBatch; u++) {
+      const int p = p0 + u, which = p >= passes_q, h = head_of(p, which);
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = x[j] * scale * w[j];
+      for (int j = 0; j < 8; j++) x[u][j] = 0.f;
+      if (p < p1 && in && h < a.heads[which])
+        load8<DT, VEC>(a.x[which], t * a.in_stride[which] + (long long)h * a.head_dim + e0, x[u]);
+    }
+  };
+  int p0 = (int)((long long)part * passes / a.splits);
+  load(p0);
+  float w[2][8] = {};
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+    if (a.weight[k] && in) load8<DT, false>(a.weight[k], e0, w[k]);
+  for (int i = lane; i < a.half; i += 64) {
+    float c, s;
+    turn(pos, a.inv_freq[i], c, s);
+    s_turn[wave][i] = make_float2(c, s);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  float c[NT], s[NT];
+#pragma unroll
+  for (int j = 0; j < NT; j++) {
+    const int e = PARTNER == kNeighbour ? e0 + 2 * j : e0 + j;
+    const int i = PARTNER == kNeighbour ? e >> 1 : (e < a.half ? e : e - a.half);
+    c[j] = 1.f;
+    s[j] = 0.f;
+    if (e < a.rot) {
+      const float2 v = s_turn[wave][i];
+      c[j] = v.x;
+      s[j] = PARTNER != kNeighbour && e < a.half ? -v.y : v.y;  // the sign of the partner's part
     }
   }
-  float y[8];
-  if constexpr (PAIRS) {
+  for (;;) {
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float c = 1.f, s = 0.f;
-      if (e0 + j < a.rot) turn(pos, a.inv_freq[(e0 + j) >> 1], c, s);
-      y[j] = x[j] * c - x[j + 1] * s;
-      y[j + 1] = x[j + 1] * c + x[j] * s;
-    }
-  } else {
-    // the row through LDS: the partner can be any element of it
-    float *mine = s_row + (tid - l) * 8;
+    for (int u = 0; u < kBatch; u++) {
+      const int p = p0 + u;
+      if (p >= p1) break;  // uniform
+      const int which = p >= passes_q, h = head_of(p, which);
+      if (a.weight[which]) {
+        float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) mine[e0 + j] = x[j];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        for (int j = 0; j < 8; j++) ss = __builtin_fmaf(x[u][j], x[u][j], ss);
+        const float scale = 1.0f / sqrtf(__builtin_fmaf(row_sum<LPR>(ss), a.inv_dim, a.eps));
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int e = e0 + j;
-      y[j] = x[j];
-      if (e < a.rot) {
-        const bool second = e >= a.half;
-        const int i = second ? e - a.half : e;
-        float c, s;
-        turn(pos, a.inv_freq[i], c, s);
-        const float other = mine[second ? i : i + a.half];
-        y[j] = second ? x[j] * c + other * s : x[j] * c - other * s;
+        for (int j = 0; j < 8; j++) x[u][j] = x[u][j] * scale * w[which][j];
       }
+      float y[8];
+      if constexpr (PARTNER == kNeighbour) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          y[2 * j] = x[u][2 * j] * c[j] - x[u][2 * j + 1] * s[j];
+          y[2 * j + 1] = x[u][2 * j + 1] * c[j] + x[u][2 * j] * s[j];
+        }
+      } else if constexpr (PARTNER == kHalfRow) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = x[u][j] * c[j] + lane_xor<LPR / 2>(x[u][j]) * s[j];
+      } else {
+        float *mine = s_row[wave] + r * (8 * LPR);
+        __builtin_amdgcn_wave_barrier();
+        reinterpret_cast<float4 *>(mine + e0)[0] = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+        reinterpret_cast<float4 *>(mine + e0)[1] = make_float4(x[u][4], x[u][5], x[u][6], x[u][7]);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int e = e0 + j, o = e >= a.rot ? e : (e < a.half ? e + a.half : e - a.half);
+          y[j] = x[u][j] * c[j] + mine[o] * s[j];
+        }
+      }
+      if (in && h < a.heads[which])
+        store8<DT, VEC>(a.out[which], t * a.out_stride[which] + (long long)h * a.head_dim + e0, y);
     }
+    p0 += kBatch;
+    if (p0 >= p1) break;
+    load(p0);
   }
-  if (in) store8<DT, VEC>(a.out[which], t * a.out_stride[which] + (long long)hh * a.head_dim + e0, y);
 }
 
 }  // namespace
@@ -228,20 +280,24 @@ extern "C" int tq_qk_norm_rope(const void *q, long long q_stride, const void *k,
   const int size = tqh::dtype_size(dtype);
   const bool vec = (!num_heads || (tqh::rows_aligned(q, q_stride, size) && tqh::rows_aligned(q_out, q_out_stride, size))) &&
                    (!num_kv_heads || (tqh::rows_aligned(k, k_stride, size) && tqh::rows_aligned(k_out, k_out_stride, size)));
-  const int lpr = head_dim <= 32 ? 4 : (head_dim <= 64 ? 8 : (head_dim <= 128 ? 16 : 32));
-  const long long blocks = (rows * lpr + 255) / 256;
+  const int lpr = head_dim <= 32 ? 4 : (head_dim <= 64 ? 8 : (head_dim <= 128 ? 16 : 32)), rpw = 64 / lpr;
+  const int passes = (num_heads + rpw - 1) / rpw + (num_kv_heads + rpw - 1) / rpw;
+  // few tokens: their rows are shared out until the card has waves enough
+  a.splits = (int)std::min<long long>(passes, std::max<long long>(1, kWaves / tokens));
+  const long long blocks = ((long long)tokens * a.splits + 3) / 4;
   if (blocks >= 1ll << 24) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "too many rows in one call");
   auto go = [&](auto l, auto d, auto v, auto p) {
     hipLaunchKernelGGL((qk_norm_rope_kernel<l.value, d.value, v.value, p.value>), dim3((unsigned)blocks), dim3(256), 0,
                        stream, a);
   };
-  auto by_pairs = [&](auto l, auto d, auto v) {
-    if (interleaved) go(l, d, v, std::true_type{});
-    else go(l, d, v, std::false_type{});
+  auto by_partner = [&](auto l, auto d, auto v) {
+    if (interleaved) go(l, d, v, std::integral_constant<int, kNeighbour>{});
+    else if (rot_dim == 8 * lpr) go(l, d, v, std::integral_constant<int, kHalfRow>{});
+    else go(l, d, v, std::integral_constant<int, kAny>{});
   };
   auto by_vec = [&](auto l, auto d) {
-    if (vec) by_pairs(l, d, std::true_type{});
-    else by_pairs(l, d, std::false_type{});
+    if (vec) by_partner(l, d, std::true_type{});
+    else by_partner(l, d, std::false_type{});
   };
   auto by_type = [&](auto l) {
     if (dtype == kF32) by_vec(l, std::integral_constant<int, kF32>{});

@@ -23,29 +23,38 @@ def _device() -> int:
     return _cur_device() if _cur_device is not None else torch.cuda.current_device()
 
 
-def _ptr(t: torch.Tensor, dtype: torch.dtype, shape, what: str) -> int:
-    """The address of a contiguous tensor of this type and shape on the current device."""
+def _refuse(t: torch.Tensor, dtype: torch.dtype, shape, what: str) -> None:
     if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{what} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
-    dev = t.get_device()
-    if dev < 0 or dev != _device():
+    if t.get_device() < 0 or t.get_device() != _device():
         raise ValueError(f"{what} must be on the current device")
-    if not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{what} must be contiguous")
 
 
-def _rows(t: torch.Tensor, what: str) -> Tuple[int, int]:
-    """Address and row stride (elements) of t [tokens, heads, head_dim], heads adjacent."""
-    n, h, d = t.shape
-    if t.dtype not in _DT:
-        raise ValueError(f"{what} must be f32/bf16/f16")
-    dev = t.get_device()
-    if dev < 0 or dev != _device():
-        raise ValueError(f"{what} must be on the current device")
-    if (t.stride(2) != 1 and d > 1) or (t.stride(1) != d and h > 1):
+# A call's checks are most of its host time (a launch takes 3 us, a comparison
+# of a tensor's attribute 0.1): one condition for a good tensor, its address
+# with it, and what is wrong with a bad one found out afterwards.
+def _ptr(t: torch.Tensor, dtype: torch.dtype, shape, what: str, dev: int) -> int:
+    """The address of a contiguous tensor of this type and shape on the current device `dev`."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(t, dtype, shape, what)
+
+
+def _rows(t: torch.Tensor, dtype: torch.dtype, shape, what: str, dev: int) -> Tuple[int, int]:
+    """Address and row stride (elements) of t [tokens, heads, head_dim], heads adjacent, likewise."""
+    n, h, d = shape
+    s0, s1, s2 = t.stride()
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev:
+        if s2 == 1 and (s1 == d or h == 1):
+            return t.data_ptr(), s0 if n > 1 else h * d
         raise ValueError(f"{what}'s heads must be adjacent (strides {t.stride()} of {list(t.shape)})")
-    return t.data_ptr(), t.stride(0) if n > 1 else h * d
+    _refuse(t, dtype, shape, what)
+
+
+def _current() -> int:
+    """The current device; -1 without one (no tensor is there)."""
+    return _device() if torch.cuda.is_initialized() else -2
 
 
 class PagedLayer:
@@ -67,15 +76,15 @@ class PagedLayer:
         self.packed_dim, self.head_dim = k_idx.shape[3], 32 * k_sc.shape[3]
         self.k_idx, self.k_sc, self.v_idx, self.v_sc, self.signs, self.norms = k_idx, k_sc, v_idx, v_sc, signs, norms
         idx, sc = (*base, self.packed_dim), (*base, self.head_dim // 32)
-        self.device = k_idx.get_device()
-        self._ptrs = (_ptr(k_idx, torch.uint8, idx, "k_idx"), _ptr(k_sc, torch.int16, sc, "k_sc"),
-                      _ptr(v_idx, torch.uint8, idx, "v_idx"), _ptr(v_sc, torch.int16, sc, "v_sc"))
+        self.device = dev = _current()
+        self._ptrs = (_ptr(k_idx, torch.uint8, idx, "k_idx", dev), _ptr(k_sc, torch.int16, sc, "k_sc", dev),
+                      _ptr(v_idx, torch.uint8, idx, "v_idx", dev), _ptr(v_sc, torch.int16, sc, "v_sc", dev))
         self._sketch = (None, None)
         if (signs is None) != (norms is None):
             raise ValueError("signs and norms come together")
         if signs is not None:
-            self._sketch = (_ptr(signs, torch.uint8, (*base, self.head_dim // 8), "signs"),
-                            _ptr(norms, torch.int16, base, "norms"))
+            self._sketch = (_ptr(signs, torch.uint8, (*base, self.head_dim // 8), "signs", dev),
+                            _ptr(norms, torch.int16, base, "norms", dev))
 
     @staticmethod
     def empty(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, bits: int, qjl: bool = False,
@@ -95,9 +104,9 @@ class PagedLayer:
         return sum(t.numel() * t.element_size() for t in (self.k_idx, self.k_sc, self.v_idx, self.v_sc, self.signs,
                                                           self.norms) if t is not None)
 
-    def _check(self, bits: int, sign_matrix: Optional[torch.Tensor]):
+    def _check(self, bits: int, sign_matrix: Optional[torch.Tensor], dev: int):
         """(signs, norms, sign matrix) addresses of a call; a sign matrix selects TQ."""
-        if self.device != _device():
+        if self.device != dev:
             raise ValueError("the layer's pages must be on the current device")
         if 8 * self.packed_dim != self.head_dim * bits:
             raise ValueError(f"the layer holds records of {self.packed_dim} bytes, not {bits}-bit ones of head_dim "
@@ -107,7 +116,7 @@ class PagedLayer:
         if self.signs is None:
             raise ValueError("a sign matrix needs pages with signs and norms")
         words = self.head_dim * self.head_dim // 32
-        return (*self._sketch, _ptr(sign_matrix, torch.int32, (words,), "sign_matrix"))
+        return (*self._sketch, _ptr(sign_matrix, torch.int32, (words,), "sign_matrix", dev))
 
 
 class PagePlan(NamedTuple):
@@ -134,24 +143,24 @@ def paged_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     free_count_out may be the inputs; new tensors by default."""
     if kv_lens.dim() != 1 or block_table.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("kv_lens [batch], block_table [batch, width] and free_pages [capacity] are expected")
-    b, i32, dev = kv_lens.shape[0], torch.int32, kv_lens.device
-    width, cap = block_table.shape[1], free_pages.shape[0]
-    ins = (_ptr(kv_lens, i32, (b,), "kv_lens"), _ptr(new_lens, i32, (b,), "new_lens"),
-           _ptr(block_table, i32, (b, width), "block_table"), _ptr(free_pages, i32, (cap,), "free_pages"),
-           _ptr(free_count, i32, (1,), "free_count"))
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    positions, starts, appended = torch.empty(num_tokens + 2 * b + 1, dtype=i32, device=dev).split(
-        (num_tokens, b + 1, b))
+    lens, i32, dev = kv_lens.shape, torch.int32, _current()
+    b, width, cap = lens[0], block_table.shape[1], free_pages.shape[0]
+    ins = (_ptr(kv_lens, i32, lens, "kv_lens", dev), _ptr(new_lens, i32, lens, "new_lens", dev), b,
+           _ptr(block_table, i32, (b, width), "block_table", dev), width,
+           _ptr(free_pages, i32, (cap,), "free_pages", dev), cap, _ptr(free_count, i32, (1,), "free_count", dev))
+    slots = kv_lens.new_empty(num_tokens, dtype=torch.int64)
+    rows = kv_lens.new_empty(num_tokens + 2 * b + 1)
+    first = rows.data_ptr()
+    positions, starts, appended = rows.split((num_tokens, b + 1, b))
     if kv_lens_out is None:
         kv_lens_out = torch.empty_like(kv_lens)
     if free_count_out is None:
         free_count_out = torch.empty_like(free_count)
-    check(lib.tq_paged_plan(ins[0], ins[1], b, ins[2], width, ins[3], cap, ins[4], page_size, num_tokens,
-                            slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), appended.data_ptr(),
-                            _ptr(kv_lens_out, i32, (b,), "kv_lens_out"),
-                            _ptr(free_count_out, i32, (1,), "free_count_out"), _stream()))
+    check(lib.tq_paged_plan(*ins, page_size, num_tokens, slots.data_ptr(), first, first + 4 * num_tokens,
+                            first + 4 * (num_tokens + b + 1), _ptr(kv_lens_out, i32, lens, "kv_lens_out", dev),
+                            _ptr(free_count_out, i32, (1,), "free_count_out", dev), _stream()))
     return PagePlan(slots, positions, starts, appended, kv_lens_out, free_count_out)
 
 
@@ -164,21 +173,26 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     (views of a fused projection); positions int32 [tokens], rows of negative
     ones left as they are in the outputs; inv_freq f32 [rot_dim / 2].  Returns
     (q, k) in new contiguous tensors, or `out` (which may be (q, k))."""
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype:
-        raise ValueError("q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] of one type are expected")
-    t, h, d = q.shape
+    qs, ks, dt = q.shape, k.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2] or k.dtype is not dt or dt not in _DT:
+        raise ValueError("q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] of one type (f32/bf16/f16) "
+                         "are expected")
+    (t, h, d), hk, dev = qs, ks[1], _current()
+    qp, q0 = _rows(q, dt, qs, "q", dev)
+    kp, k0 = _rows(k, dt, ks, "k", dev)
     if out is None:
-        out = torch.empty((t, h, d), dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    qo, ko = out
-    if qo.shape != q.shape or ko.shape != k.shape or qo.dtype != q.dtype or ko.dtype != k.dtype:
-        raise ValueError("out must have q's and k's shapes and type")
-    (qp, qs), (kp, ks), (qop, qos), (kop, kos) = _rows(q, "q"), _rows(k, "k"), _rows(qo, "out[0]"), _rows(ko, "out[1]")
-    wq = None if q_weight is None else _ptr(q_weight, q.dtype, (d,), "q_weight")
-    wk = None if k_weight is None else _ptr(k_weight, q.dtype, (d,), "k_weight")
-    check(lib.tq_qk_norm_rope(qp, qs, kp, ks, _DT[q.dtype], _ptr(positions, torch.int32, (t,), "positions"), t, h,
-                              k.shape[1], d, _ptr(inv_freq, torch.float32, (inv_freq.numel(),), "inv_freq"),
-                              2 * inv_freq.numel(), 1 if interleaved else 0, wq, wk, eps, qop, qos, kop, kos,
-                              _stream()))
+        qo, ko = q.new_empty(qs), k.new_empty(ks)
+        qop, qo0, kop, ko0 = qo.data_ptr(), h * d, ko.data_ptr(), hk * d
+    else:
+        qo, ko = out
+        qop, qo0 = _rows(qo, dt, qs, "out[0]", dev)
+        kop, ko0 = _rows(ko, dt, ks, "out[1]", dev)
+    half = inv_freq.numel()
+    wq = None if q_weight is None else _ptr(q_weight, dt, (d,), "q_weight", dev)
+    wk = None if k_weight is None else _ptr(k_weight, dt, (d,), "k_weight", dev)
+    check(lib.tq_qk_norm_rope(qp, q0, kp, k0, _DT[dt], _ptr(positions, torch.int32, (t,), "positions", dev), t, h, hk,
+                              d, _ptr(inv_freq, torch.float32, (half,), "inv_freq", dev), 2 * half,
+                              1 if interleaved else 0, wq, wk, eps, qop, qo0, kop, ko0, _stream()))
     return qo, ko
 
 
@@ -189,16 +203,15 @@ def paged_store(layer: PagedLayer, slots: torch.Tensor, k: torch.Tensor, v: torc
     into the records of slots int64 [tokens]; rows whose slot is outside the
     pages are skipped, the others' slots are distinct.  sign_matrix: TQ records,
     whose keys are sketched too."""
-    t = slots.shape[0]
-    shape = (t, layer.num_kv_heads, layer.head_dim)
-    if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
-        raise ValueError(f"k and v must be {list(shape)} of one type, got {list(k.shape)} and {list(v.shape)}")
-    sg, nm, rm = layer._check(bits, sign_matrix)
-    (kp, ks), (vp, vs) = _rows(k, "k"), _rows(v, "v")
-    ki, ksc, vi, vsc = layer._ptrs
-    check(lib.tq_paged_store(kp, ks, vp, vs, _DT[k.dtype], _ptr(slots, torch.int64, (t,), "slots"), t, ki, ksc, vi,
-                             vsc, sg, nm, rm, layer.num_pages, layer.num_kv_heads, layer.page_size, layer.head_dim,
-                             bits, outlier_blocks, norm_mode, _stream()))
+    t, hk, d, dt, dev = slots.shape[0], layer.num_kv_heads, layer.head_dim, k.dtype, _current()
+    if dt not in _DT or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("k and v [tokens, num_kv_heads, head_dim] must be f32/bf16/f16")
+    sg, nm, rm = layer._check(bits, sign_matrix, dev)
+    kp, k0 = _rows(k, dt, (t, hk, d), "k", dev)
+    vp, v0 = _rows(v, dt, (t, hk, d), "v", dev)
+    check(lib.tq_paged_store(kp, k0, vp, v0, _DT[dt], _ptr(slots, torch.int64, (t,), "slots", dev), t, *layer._ptrs,
+                             sg, nm, rm, layer.num_pages, hk, layer.page_size, d, bits, outlier_blocks, norm_mode,
+                             _stream()))
 
 
 def paged_load(layer: PagedLayer, slots: torch.Tensor, bits: int, outlier_blocks: int = TQ_OUTLIER_ALL,
@@ -207,19 +220,17 @@ def paged_load(layer: PagedLayer, slots: torch.Tensor, bits: int, outlier_blocks
     """The records of slots int64 [tokens] as activations: (k, v) [tokens,
     num_kv_heads, head_dim] in out_dtype, or into `out`; rows whose slot is
     outside the pages are left as they are."""
-    t = slots.shape[0]
-    shape = (t, layer.num_kv_heads, layer.head_dim)
+    shape, dev = (slots.shape[0], layer.num_kv_heads, layer.head_dim), _current()
+    layer._check(bits, None, dev)
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=slots.device), torch.empty(shape, dtype=out_dtype,
-                                                                                    device=slots.device)
+        out = slots.new_empty(shape, dtype=out_dtype), slots.new_empty(shape, dtype=out_dtype)
     k, v = out
-    if k.dtype not in _DT:
+    dt = k.dtype
+    if dt not in _DT:
         raise ValueError("out must be f32/bf16/f16")
-    layer._check(bits, None)
-    check(lib.tq_paged_load(*layer._ptrs, _ptr(slots, torch.int64, (t,), "slots"), t, layer.num_pages,
-                            layer.num_kv_heads, layer.page_size, layer.head_dim, bits, outlier_blocks, norm_mode,
-                            _ptr(k, k.dtype, shape, "out[0]"), _ptr(v, k.dtype, shape, "out[1]"), _DT[k.dtype],
-                            _stream()))
+    check(lib.tq_paged_load(*layer._ptrs, _ptr(slots, torch.int64, shape[:1], "slots", dev), shape[0], layer.num_pages,
+                            shape[1], layer.page_size, shape[2], bits, outlier_blocks, norm_mode,
+                            _ptr(k, dt, shape, "out[0]", dev), _ptr(v, dt, shape, "out[1]", dev), _DT[dt], _stream()))
     return k, v
 
 
@@ -234,21 +245,22 @@ def paged_decode_attention(q: torch.Tensor, layer: PagedLayer, block_table: torc
     QJL correction of the logits.  workspace: an AttentionWorkspace of at least
     this batch, heads and max_kv_len; one call at a time uses it.  Returns
     [batch, heads, head_dim] in out_dtype (q's by default)."""
-    b, h, d = q.shape
-    if d != layer.head_dim or block_table.dim() != 2:
+    shape, dt, dev = q.shape, q.dtype, _current()
+    if len(shape) != 3 or shape[2] != layer.head_dim or block_table.dim() != 2:
         raise ValueError(f"q [batch, heads, {layer.head_dim}] and block_table [batch, width] are expected")
-    width = block_table.shape[1]
+    (b, h, d), width = shape, block_table.shape[1]
     if out is None:
-        out = torch.empty((b, h, d), dtype=out_dtype or q.dtype, device=q.device)
-    if q.dtype not in _DT or out.dtype not in _DT:
+        out = torch.empty_like(q) if out_dtype is None or out_dtype is dt else torch.empty_like(q, dtype=out_dtype)
+    odt = out.dtype
+    if dt not in _DT or odt not in _DT:
         raise ValueError("q and out must be f32/bf16/f16")
-    sg, nm, rm = layer._check(bits, sign_matrix)
+    sg, nm, rm = layer._check(bits, sign_matrix, dev)
     check(lib.tq_paged_decode_attention(
-        _ptr(q, q.dtype, (b, h, d), "q"), _DT[q.dtype], *layer._ptrs, sg, nm, rm,
-        _ptr(block_table, torch.int32, (b, width), "block_table"), width, _ptr(kv_lens, torch.int32, (b,), "kv_lens"),
-        b, h, layer.num_kv_heads, d, bits, outlier_blocks, norm_mode, layer.page_size, layer.num_pages, max_kv_len,
-        softmax_scale, _ptr(out, out.dtype, (b, h, d), "out"), _DT[out.dtype],
-        _ptr(workspace.buf, torch.uint8, (workspace.nbytes,), "workspace"), workspace.nbytes, _stream()))
+        _ptr(q, dt, shape, "q", dev), _DT[dt], *layer._ptrs, sg, nm, rm,
+        _ptr(block_table, torch.int32, (b, width), "block_table", dev), width,
+        _ptr(kv_lens, torch.int32, (b,), "kv_lens", dev), b, h, layer.num_kv_heads, d, bits, outlier_blocks, norm_mode,
+        layer.page_size, layer.num_pages, max_kv_len, softmax_scale, _ptr(out, odt, shape, "out", dev), _DT[odt],
+        _ptr(workspace.buf, torch.uint8, (workspace.nbytes,), "workspace", dev), workspace.nbytes, _stream()))
     return out
 
 
