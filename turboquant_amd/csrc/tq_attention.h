@@ -80,6 +80,7 @@ struct AttnArgs {
   int bal_nwg;
   int bal_batch;
   int bal_ny;
+  int bal_lpt;  // over pages: long ranges first
   void *out;
   int out_dtype;
   // TQ: rq [b][h][head_dim] f32 = R q (precompute_query_projections); per
@@ -125,6 +126,7 @@ struct PageArgs {
 // Sequences of a balanced split: one a lane, over pages four.
 template <bool PAGED>
 constexpr int kBalSeqs = PAGED ? 256 : 64;
+constexpr int kMinRange = 512;  // tokens of a balanced range over pages, at least
 
 // Query element as stored (f32 bits or a 16-bit pattern), converted
 // separately so that the wait for the load lands at the first use.
@@ -150,8 +152,10 @@ constexpr int dmin(int x, int y) { return x < y ? x : y; }
 // LDS of the split-K merge (merge_heads) for a workgroup of `waves` waves
 constexpr int merge_lds(int waves) { return waves * 256 * 4 + waves * 8 * 2 * 4; }
 
-template <int BITS_, int MODE_, int NQB_, int HG_, int TPW_, int WAVES_>
+// QUAD: four codes a codebook read and no remainders (tq_decode_kernel.h)
+template <int BITS_, int MODE_, int NQB_, int HG_, int TPW_, int WAVES_, bool QUAD_ = false>
 struct DecCfg {
+  static constexpr bool QUAD = QUAD_;
   static constexpr int BITS = BITS_, MODE = MODE_, NQB = NQB_, HG = HG_, TPW = TPW_, WAVES = WAVES_;
   static constexpr int CB = MODE == kModePqo ? BITS : BITS - 1;  // codebook bits
   static constexpr bool QJL = MODE == kModeTq;
@@ -163,8 +167,9 @@ struct DecCfg {
   static constexpr int HPM = 8 / QPM;
   static constexpr int QG = NQB / QPM;           // qblock groups (K) / sets (V)
   static constexpr int ES = 4 / QPM;             // parts of a qblock stream (lanes per qblock)
-  static constexpr int KJ = 2 * QPM;             // K slices (4 elements each) per group
-  static constexpr int PPL = 16 / ES;            // pairs per lane part (= V slices per set)
+  static constexpr int KJ = QUAD ? QPM : 2 * QPM;  // K slices (4 elements each, QUAD 8) per group
+  static constexpr int CPR = QUAD ? 4 : 2;         // codes a codebook read
+  static constexpr int PPL = 32 / CPR / ES;        // reads per lane part (= V slices per set)
   static constexpr int NW = ES == 1 ? QW : 2;    // record words a lane holds per group
   static constexpr int NKT = TPW / 16, NVP = TPW / 32;
   // grid V pass: the row stride (bytes) of a staged V record, padded by 8 so
@@ -175,12 +180,12 @@ struct DecCfg {
 #endif
   static constexpr int LOOKAHEAD = TQ_DECODE_LOOKAHEAD;  // load groups in flight per wave
   static constexpr int THREADS = 64 * WAVES, CHUNK = WAVES * TPW;
-  static constexpr int NPAIR = 1 << (2 * BITS);
+  static constexpr int NPAIR = 1 << (CPR * BITS);
   static constexpr int SW4 = (NQB + 3) / 4;      // QJL: sign words per lane and tile
   static constexpr int TPL = TPW / 64;           // V-scale tokens per lane
   static constexpr bool QA_REGS = QG * KJ <= 8;  // query operands in registers (else LDS)
   // LDS carve (32-bit words)
-  static constexpr int OFF_PAIR = 0;                                  // uint2 [NPAIR]
+  static constexpr int OFF_PAIR = 0;                                  // uint2 [NPAIR]: pairs, or quads
   static constexpr int OFF_NIB = OFF_PAIR + 2 * NPAIR;                // QJL uint2 [16]
   // the key-pass query operands, u32x4 [QG*KJ][64] (read per instruction,
   // or by QA_REGS configurations into registers at each chunk's K pass)
@@ -415,6 +420,8 @@ using StreamCfg4 = DecCfg<BITS, MODE, NQB, HG, stream_tpw_c(NQB, HG, MODE == kMo
 // in one round even so (a sequence's KV heads over shorter contexts)
 template <int BITS, int MODE, int NQB, int HG>
 using StreamCfg64 = DecCfg<BITS, MODE, NQB, HG, 64, 8>;
+template <int BITS, int MODE, int NQB, int HG>
+using StreamCfgQuad = DecCfg<BITS, MODE, NQB, HG, NQB <= 4 && HG <= 2 ? 128 : 64, 8, true>;
 // Compute units of the current device (cached per device).
 int device_cus();
 

@@ -99,11 +99,11 @@ __device__ __forceinline__ u32x4 nib_operand(uint32_t w) {
   return u32x4{w & 0x000F000Fu, w & 0x00F000F0u, h & 0x000F000Fu, h & 0x00F000F0u};
 }
 
-// BITS-bit code pair p of a lane's stream w (little-endian words), as the
-// byte offset of its pair-table entry (code * 8): two VALU per pair.
-template <int BITS, int NWD>
+// Read p's CODES BITS-bit codes of a lane's stream w (little-endian words), as
+// the byte offset of their table entry (codes * 8): two VALU each.
+template <int BITS, int CODES, int NWD>
 __device__ __forceinline__ uint32_t pair_off(const uint32_t (&w)[NWD], int p) {
-  constexpr int W = 2 * BITS;
+  constexpr int W = CODES * BITS;
   constexpr uint32_t M = ((1u << W) - 1u) << 3;
   const int pos = W * p;
   if (pos < 3) return (w[0] << 3) & M;
@@ -118,12 +118,12 @@ __device__ __forceinline__ uint32_t pair_off(const uint32_t (&w)[NWD], int p) {
 template <class C>
 __device__ __forceinline__ int part_word(int es) {
   if constexpr (C::ES == 1) return 0;
-  else return dmin((es * C::PPL * 2 * C::BITS) >> 5, C::QW - 2);
+  else return dmin((es * C::PPL * C::CPR * C::BITS) >> 5, C::QW - 2);
 }
 template <class C>
 __device__ __forceinline__ void align_part(uint32_t (&w)[C::NW], int es) {
   if constexpr (C::ES > 1) {
-    const int sh = es * C::PPL * 2 * C::BITS - 32 * part_word<C>(es);
+    const int sh = es * C::PPL * C::CPR * C::BITS - 32 * part_word<C>(es);
     const uint64_t x = ((((uint64_t)w[1]) << 32) | w[0]) >> sh;
     w[0] = (uint32_t)x;
     w[1] = (uint32_t)(x >> 32);
@@ -267,7 +267,7 @@ template <class C, bool INLINE_MERGE, bool GRID, bool MULTI, bool PROJ = false, 
 #ifndef TQ_DECODE_WPE
 #define TQ_DECODE_WPE 2
 #endif
-__global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kernel(const uint8_t *k_idx, const uint8_t *v_idx,
+__global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void stream_decode_kernel(const uint8_t *k_idx, const uint8_t *v_idx,
                                                                const uint16_t *k_sc, const uint16_t *v_sc,
                                                                long long seq_stride, long long kv_head_stride,
                                                                int len_hint, AttnArgs a,
@@ -293,6 +293,21 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   // grid V pass: each wave's 64-token block of V records, token-major
   __shared__ __attribute__((aligned(16))) uint8_t vstage[GRID ? C::VSTAGE : 16];
   uint2 *s_pair = reinterpret_cast<uint2 *>(lds + C::OFF_PAIR);
+  // QUAD: a table of four codes (4,096 entries of 3-bit codes, 32 KiB for eight
+  // waves) halves the codebook reads, and centroids of one f16 part halve both passes'
+  // instructions: the codebook is scaled by kQuadScale, at which its f16
+  // roundings are off by 2^-15.4 (four magnitudes; two: 2^-20) instead of up
+  // to 2^-12, an eighth of an f16 result's own rounding; f32 results take the
+  // pairs, whose two parts are exact.  The scale goes out of the query and of
+  // the value weights.  A pass is bound by the LDS (57 % of the cycles with
+  // pairs) and the vector unit (49 %); quads take 128 registers, four waves a
+  // SIMD instead of two.  128 ragged sequences of up to 8,192 tokens, 16 over 8
+  // heads, 238 -> 172 us, 64 117 -> 79, 16 of up to 16,384, 32 over 8 heads,
+  // 59.7 -> 51.8.
+  constexpr bool QUAD = C::QUAD;
+  static_assert(!QUAD || (BITS == 3 && MULTI && PAGED && !GRID), "quads: range launches over 3-bit pages");
+  constexpr float kQuadScale = QUAD ? (C::CB == 3 ? 1.8351183f : 1.8351586f) : 1.f;
+  __shared__ uint32_t s_two[QUAD ? 64 : 1];  // the f16 pairs that quads are made of
   float *s_q = lds + C::OFF_Q - LSH;
   float *s_qmax = lds + C::OFF_QMAX - LSH;
   float *s_rq = lds + C::OFF_RQ - LSH;
@@ -341,6 +356,12 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   // long sequences' ranges setting the time.  A wave holds the batch's chunk
   // counts (one sequence per lane; over pages up to four), so the split costs a few reductions and
   // a ballot, no LDS and no barrier before the first loads. ----
+  // Over pages the unit of the split is a wave's tokens of a step (TPW), not a
+  // chunk, at least kMinRange tokens a range (the workspace has room for one
+  // partial per 512): whole chunks leave up to half of the workgroups' time
+  // idle where a sequence has few.  With more ranges than fit at once (bal_lpt)
+  // long ones start first, in 16 classes of length: what starts last is short.
+  constexpr int UNIT = PAGED ? C::TPW : C::CHUNK;
   int bal_ck0 = 0, bal_nck = 0, bal_nparts = 0;
   const bool bal = MULTI && a.bal_nwg > 0;
   if constexpr (MULTI) {
@@ -353,7 +374,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
         n[k] = 0;
         if (64 * k + lane < nb) {
           const int lb = len_hint >= 0 ? len_hint : min(max(a_lens[64 * k + lane], 0), a_max);
-          n[k] = (lb + C::CHUNK - 1) / C::CHUNK;
+          n[k] = (lb + UNIT - 1) / UNIT;
         }
         T += wave_sum_i(n[k]);
         most = max(most, wave_max_i(n[k]));
@@ -368,14 +389,34 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
         for (int k = 0; k < SQ; k++) less += wave_sum_i((n[k] + S - 2) / (S - 1));
         if ((long long)less * ny <= nwg) S--;
       }
+      if constexpr (PAGED) S = max(S, kMinRange / UNIT);
       S = __builtin_amdgcn_readfirstlane(S);
       int rb[SQ], pre[SQ], ranges = 0;  // ranges per KV head of the lane's sequences, and before each
 #pragma unroll
-      for (int k = 0; k < SQ; k++) {
-        rb[k] = (n[k] + S - 1) / S;
-        const int incl = wave_incl_scan_i(rb[k]);
-        pre[k] = ranges + incl - rb[k];
-        ranges += __builtin_amdgcn_readlane(incl, 63);
+      for (int k = 0; k < SQ; k++) rb[k] = (n[k] + S - 1) / S;
+      if (PAGED && a.bal_lpt) {
+        int level[SQ];
+#pragma unroll
+        for (int k = 0; k < SQ; k++) {
+          level[k] = rb[k] ? min((int)((float)n[k] * 16.f / ((float)rb[k] * (float)S)), 15) : -1;
+          pre[k] = 0;
+        }
+        for (int lv = 15; lv >= 0; lv--)
+#pragma unroll
+          for (int k = 0; k < SQ; k++) {
+            const bool mine = level[k] == lv;
+            if (!__ballot(mine)) continue;
+            const int incl = wave_incl_scan_i(mine ? rb[k] : 0);
+            if (mine) pre[k] = ranges + incl - rb[k];
+            ranges += __builtin_amdgcn_readlane(incl, 63);
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < SQ; k++) {
+          const int incl = wave_incl_scan_i(rb[k]);
+          pre[k] = ranges + incl - rb[k];
+          ranges += __builtin_amdgcn_readlane(incl, 63);
+        }
       }
       const int wi = blockIdx.x;
       const int total = ranges * ny;
@@ -393,14 +434,15 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
         __builtin_amdgcn_s_waitcnt(0);
         return;
       }
-      // workgroup wi: sequence b (the last whose ranges start at or before
-      // it), KV head y, range r of its R_b
+      // workgroup wi: the sequence b that it lies in the ranges of, KV head y,
+      // range r of its R_b
       int pre_b = 0, r_b = 1, n_b = 0;
 #pragma unroll
       for (int k = 0; k < SQ; k++) {
-        const unsigned long long le = __ballot(64 * k + lane < nb && pre[k] * ny <= wi);
-        if (le) {
-          const int l = __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(le));
+        const unsigned long long in =
+            __ballot(64 * k + lane < nb && pre[k] * ny <= wi && wi < (pre[k] + rb[k]) * ny);
+        if (in) {
+          const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(in));
           b = 64 * k + l;
           pre_b = __builtin_amdgcn_readlane(pre[k], l);
           r_b = __builtin_amdgcn_readlane(rb[k], l);
@@ -410,7 +452,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
       const int k = wi - pre_b * ny;
       y = k / r_b;
       const int r = k - y * r_b;
-      bal_ck0 = (int)((long long)r * n_b / r_b);
+      bal_ck0 = (int)((long long)r * n_b / r_b);  // in units
       bal_nck = (int)((long long)(r + 1) * n_b / r_b) - bal_ck0;
       bal_nparts = r_b;
       c = r;
@@ -487,7 +529,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   const int nchunks = (len + C::CHUNK - 1) / C::CHUNK;
   const int cpr = a_cpr;
   const int ck0 = bal ? bal_ck0 : c * cpr;
-  if (ck0 >= nchunks) {  // an empty range is not counted by the merge
+  if ((!PAGED || !bal) && ck0 >= nchunks) {  // an empty range is not counted by the merge
     if (len == 0 && c == 0) {
       // an empty sequence attends to nothing: zero output (cuda/attention.rs:65-68)
       for (int e = tid; e < nh * HD; e += C::THREADS) {
@@ -499,7 +541,14 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     __builtin_amdgcn_s_waitcnt(0);
     return;
   }
-  const int nck = bal ? bal_nck : (MULTI ? min(cpr, nchunks - ck0) : 1);  // chunks of this range
+  // the range's first token and the end of its tokens, and its chunks; over
+  // pages those in which this wave has tokens (the others leave the compute
+  // unit to other workgroups)
+  const int tok0 = PAGED && bal ? bal_ck0 * UNIT : ck0 * C::CHUNK;
+  const int lim = PAGED && bal ? min(len, (bal_ck0 + bal_nck) * UNIT)
+                               : (PAGED && MULTI ? min(len, (ck0 + cpr) * C::CHUNK) : len);
+  const int nck = PAGED && MULTI ? max((lim - tok0 - wave * TPW + C::CHUNK - 1) / C::CHUNK, 0)
+                                 : (bal ? bal_nck : (MULTI ? min(cpr, nchunks - ck0) : 1));
   const int nparts = bal ? bal_nparts : (nchunks + cpr - 1) / cpr;      // ranges the merge folds
 
   // ---- records.  Wave w's tokens of a chunk start at tw = chunk CHUNK +
@@ -520,7 +569,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   const uint32_t kvo = (uint32_t)l16 * PACKED + (uint32_t)(kqb * QW + part_word<C>(kes)) * 4u;
   const uint32_t kso = ((uint32_t)l16 * NQB + kqb) * 2u;
   const uint32_t vvo = (uint32_t)(4 * lg + (l16 >> 2)) * PACKED + (uint32_t)(vqb * QW + part_word<C>(ves)) * 4u;
-  const uint32_t tw_first = (uint32_t)(ck0 * C::CHUNK + wave * TPW);
+  const uint32_t tw_first = (uint32_t)(tok0 + wave * TPW);
   uint32_t kw[NKT][QG][NW], vw[GRID ? 1 : NKT][QG][NW];
   uint32_t vg[GRID ? NKT : 1][NQB];  // grid V pass: lane l's 4 NQB bytes of its tile
   uint32_t ksv[NKT][QG];
@@ -537,7 +586,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   auto gather_pages = [&](uint32_t tw0) -> int {
     if constexpr (PAGED) {
       const int t = (int)tw0 + C::TPL * lane;
-      return t < len ? ap.table[(long long)b * ap.width + (t >> ap.shift)] : -1;
+      return t < lim ? ap.table[(long long)b * ap.width + (t >> ap.shift)] : -1;
     } else {
       return -1;
     }
@@ -557,7 +606,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     else return 0;
   };
   auto tile_count = [&](int i, uint32_t t16) -> int {
-    if constexpr (PAGED) return pages[i] < 0 ? 0 : min(max(len - (int)t16, 0), 16);
+    if constexpr (PAGED) return pages[i] < 0 ? 0 : min(max(lim - (int)t16, 0), 16);
     else return 0;
   };
   // The wave's loads form one stream of groups, consumed in order: K tile i
@@ -601,7 +650,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
 #pragma unroll
           for (int j = 0; j < (NQB + 1) / 2; j++) vsr[u][j] = 0u;
         const int t = (int)tw0 + C::TPL * lane;
-        if (vpage >= 0 && t < len) {
+        if (vpage >= 0 && t < lim) {
           const uint16_t *p = v_sc + ((((long long)vpage * a.num_kv_heads + g) << ap.shift) + (t & ((1 << ap.shift) - 1))) * NQB;
 #pragma unroll
           for (int u = 0; u < C::TPL; u++) {
@@ -658,7 +707,9 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
 #endif
   // LA0 K tiles go out with the first chunk's prologue (more would hold the
   // waves at issue before their setup), LA during the K passes
-  constexpr int LA = dmin(MULTI ? TQ_DECODE_LOOKAHEAD_MULTI : TQ_DECODE_LOOKAHEAD_PASS, NKT);
+  // QUAD: two tiles ahead (128 registers, four waves a SIMD; four ahead spill
+  // and measured the same, 78 us against 82 at 64 sequences)
+  constexpr int LA = dmin(QUAD ? 2 : (MULTI ? TQ_DECODE_LOOKAHEAD_MULTI : TQ_DECODE_LOOKAHEAD_PASS), NKT);
   constexpr int LA0 = MULTI ? LA : dmin(C::LOOKAHEAD, LA);
   constexpr int VP_NEXT = NVP >= 2 ? NVP - 2 : 0;
   auto issue_first = [&](uint32_t tw0, int n) {
@@ -697,8 +748,12 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   };
   // ---- pair table (the caller's device codebook, L2Norm tables from the
   // arguments, or the PQO constants) ----
-  static_assert(C::NPAIR <= 256, "one pair-table entry per lane");
-  if (!GRID && tid < C::NPAIR) {  // the grid passes read no table (its words hold the query operands)
+  static_assert(QUAD || C::NPAIR <= 256, "one pair-table entry per lane");
+  if constexpr (QUAD) {
+    if (tid < 64)
+      s_two[tid] = (uint32_t)f32_to_f16(pqo_centroid<C::CB>(pi0) * kQuadScale) |
+                   ((uint32_t)f32_to_f16(pqo_centroid<C::CB>(pi1) * kQuadScale) << 16);
+  } else if (!GRID && tid < C::NPAIR) {  // the grid passes read no table (its words hold the query operands)
     const int e = tid, i0 = pi0, i1 = pi1;
     float c0, c1;
     if (a.cb_dev) {
@@ -798,7 +853,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   }
   // ---- rotated, scaled query: 32-lane butterflies (elements of a qblock sit
   // in 32 consecutive lanes; absent heads are whole zero blocks) ----
-  const float qscale = a.softmax_scale * kLog2e * kInvSqrt32;
+  const float qscale = a.softmax_scale * kLog2e * kInvSqrt32 * (1.f / kQuadScale);
   const float qsign = a.sg_dev ? sgl : decode_sign(tid & 31);
 #pragma unroll
   for (int k = 0; k < QIT; k++) {
@@ -854,7 +909,16 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   auto make_qa = [&](int qg, int j, int m, int kg) -> u32x4 {
     const int qbl = m / (2 * HPM), hl = (m >> 1) % HPM, part = m & 1;
     u32x4 val = {0u, 0u, 0u, 0u};
-    if (kg / ES == qbl && hl < nh) {
+    if (QUAD && kg / ES == qbl && hl < nh) {  // eight elements, 8 j on
+      const float sc = exp2i(-head_exp(s_qmax, hl));
+      const float *src = s_q + hl * HD + (qg * QPM + qbl) * 32 + (kg % ES) * (32 / ES) + 8 * j;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float x0 = src[2 * i] * sc, x1 = src[2 * i + 1] * sc;
+        const float h0 = split_hi(x0), h1 = split_hi(x1);
+        val[i] = part ? pack_f16(x0 - h0, x1 - h1) : pack_f16(h0, h1);
+      }
+    } else if (kg / ES == qbl && hl < nh) {
       const float sc = exp2i(-head_exp(s_qmax, hl));
       const float4 q4 = *reinterpret_cast<const float4 *>(s_q + hl * HD + (qg * QPM + qbl) * 32 +
                                                           (kg % ES) * (32 / ES) + 4 * j);
@@ -892,6 +956,8 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     }
     return val;
   };
+  if constexpr (QUAD)
+    for (int e = tid; e < C::NPAIR; e += C::THREADS) s_pair[e] = make_uint2(s_two[e & 63], s_two[e >> 6]);
   // each operand is the same for every wave: the workgroup's lanes build
   // them once
   for (int e = tid; e < QG * KJA * 64; e += C::THREADS) {
@@ -985,7 +1051,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   }
   int evrun = 0;
   for (int ck = 0; ck < nck; ck++) {
-  const int tw = (ck0 + ck) * C::CHUNK + wave * TPW;
+  const int tw = tok0 + ck * C::CHUNK + wave * TPW;
   const uint32_t tw0 = (uint32_t)tw;
   if constexpr (PAGED && MULTI) {
     if (ck + 1 < nck) vpage_next = gather_pages(tw0 + C::CHUNK);
@@ -1031,7 +1097,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
 #pragma unroll
       for (int j = 0; j < 2 * KJ; j++)
         e[qg][j >> 1][j & 1] = *reinterpret_cast<const uint2 *>(reinterpret_cast<const char *>(s_pair) +
-                                                                pair_off<BITS, NW>(kw[i][qg], j));
+                                                                pair_off<BITS, C::CPR, NW>(kw[i][qg], j));
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int qg = 0; qg < QG; qg++)
@@ -1120,7 +1186,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     for (int qb = 0; qb < NQB; qb++) {
       const uint32_t bits = NQB == 1 ? vsr[u][0] : (vsr[u][qb >> 1] >> (16 * (qb & 1)));
       svv[u][qb] = fabsf(f16_to_f32((uint16_t)(bits & 0xffffu)));
-      if (PAGED && u > 0 && tw + C::TPL * lane + u >= len) svv[u][qb] = 0.f;  // what lies behind the last token
+      if (PAGED && u > 0 && tw + C::TPL * lane + u >= lim) svv[u][qb] = 0.f;  // what lies behind the last token
       smax = fmaxf(smax, svv[u][qb]);
     }
   // the running exponent Ev is the largest of the range's chunks so far; the
@@ -1129,7 +1195,7 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
   const int ev = ck == 0 ? evc : max(evrun, evc);
   const float beta = ck == 0 ? 0.f : exp2i(evrun - ev);
   evrun = ev;
-  const float vinv = exp2i(-ev);
+  const float vinv = exp2i(-ev) * (1.f / kQuadScale);
 #pragma unroll
   for (int u = 0; u < C::TPL; u++)
 #pragma unroll
@@ -1303,8 +1369,8 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
       u32x2 r[PPL][2];
 #pragma unroll
       for (int j = 0; j < PPL; j++) {
-        r[j][0] = lds_read_tr16(reinterpret_cast<const char *>(s_pair) + pair_off<BITS, NW>(vw[2 * vp][vs], j));
-        r[j][1] = lds_read_tr16(reinterpret_cast<const char *>(s_pair) + pair_off<BITS, NW>(vw[2 * vp + 1][vs], j));
+        r[j][0] = lds_read_tr16(reinterpret_cast<const char *>(s_pair) + pair_off<BITS, C::CPR, NW>(vw[2 * vp][vs], j));
+        r[j][1] = lds_read_tr16(reinterpret_cast<const char *>(s_pair) + pair_off<BITS, C::CPR, NW>(vw[2 * vp + 1][vs], j));
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1323,6 +1389,22 @@ __global__ __launch_bounds__(C::THREADS, TQ_DECODE_WPE) void stream_decode_kerne
     for (int vs = 0; vs < QG; vs++)
 #pragma unroll
       for (int j = 0; j < PPL; j++) {
+        if constexpr (QUAD) {  // four elements a slice
+          float o[4];
+#pragma unroll
+          for (int cc = 0; cc < 4; cc++) {
+            const float xx = dv[vs][j][cc];
+            o[cc] = dpp_quad_xor1(xx) + xx;
+            asm volatile("" : "+v"(o[cc]));  // keeps the add beside its DPP read
+          }
+          if (keep) {
+            float4 *dst = reinterpret_cast<float4 *>(comb + hv * HD + (vs * QPM + oqb) * 32 + 4 * (ops * PPL + j));
+            const float4 old = *dst;
+            *dst = make_float4(__builtin_fmaf(old.x, rf, o[0]), __builtin_fmaf(old.y, rf, o[1]),
+                               __builtin_fmaf(old.z, rf, o[2]), __builtin_fmaf(old.w, rf, o[3]));
+          }
+          continue;
+        }
         float o[2];
 #pragma unroll
         for (int cc = 0; cc < 2; cc++) {
@@ -1518,9 +1600,20 @@ void launch_stream_k(AttnArgs &a, dim3 grid, hipStream_t st, int len_hint, X *ap
     if (a.bal_nwg < 0) {
       // balanced split: as many workgroups as the compute units hold at once,
       // at most one per task and at least one per (sequence, KV head) pair
+      // (over pages three tenths more where the pairs fill half to all of a
+      // round: one round of whole pairs is as long as its longest.  Ragged 3-bit
+      // batches of 40, 48, 56 and 64 sequences over 8 KV heads, 512 workgroups
+      // at once: 74.1, 67.4, 76.1, 78.0 -> 45.8, 54.4, 68.2, 71.9 us; 32, 72, 96
+      // and 128 sequences are slower so, 46.5 -> 49.0, 85.5 -> 87.0, 108.5 ->
+      // 112.1, 157.4 -> 161.1 us)
       const long long pairs = (long long)a.bal_batch * a.bal_ny;
-      a.bal_nwg = (int)min((long long)-a.bal_nwg,
-                           max((long long)resident_workgroups<kernel, C::THREADS>() * device_cus(), pairs));
+      const long long room = (long long)resident_workgroups<kernel, C::THREADS>() * device_cus();
+      long long want = max(room, pairs);
+      if constexpr (PAGED) {
+        if (2 * pairs > room && pairs <= room + room / 8) want += want * 3 / 10;
+        a.bal_lpt = want > room;
+      }
+      a.bal_nwg = (int)min((long long)-a.bal_nwg, want);
       grid = dim3((unsigned)a.bal_nwg, 1u, 1u);
     }
     if constexpr (PAGED)
@@ -1587,10 +1680,11 @@ void launch_stream_c(AttnArgs &a, dim3 grid, hipStream_t st, X *ap) {
   grid.x = (unsigned)((chunks + a.cpr - 1) / a.cpr);
   if (grid.x == 0) grid.x = 1;  // an empty batch still zeroes its outputs
   const int len_hint = a.kv_lens ? -1 : max(a.single_len, 0);
-  if constexpr (INLINE || C::CHUNK < kRefPartition) {
+  if constexpr (C::QUAD) return launch_stream_k<C, INLINE, true>(a, grid, st, len_hint, ap);
+  else if constexpr (INLINE || C::CHUNK < kRefPartition) {
     if (a.cpr > 1) return launch_stream_k<C, INLINE, true>(a, grid, st, len_hint, ap);
   }
-  launch_stream_k<C, INLINE, false>(a, grid, st, len_hint, ap);
+  if constexpr (!C::QUAD) launch_stream_k<C, INLINE, false>(a, grid, st, len_hint, ap);
 }
 // The cache decode picks the workgroup size per launch: 8 waves while the
 // grid of 8-wave workgroups leaves compute units idle (one long sequence:
@@ -1602,6 +1696,12 @@ void launch_stream_cfg(AttnArgs &a, dim3 grid, hipStream_t st, X *ap) {
   using C = StreamCfg<BITS, MODE, NQB, HG>;
   using C4 = StreamCfg4<BITS, MODE, NQB, HG>;
   using C64 = StreamCfg64<BITS, MODE, NQB, HG>;
+  using CQ = StreamCfgQuad<BITS, MODE, NQB, HG>;
+  if constexpr (std::is_same_v<X, PageArgs> && BITS == 3 && CQ::TOTAL * 4 + CQ::MERGE_LDS + 512 <= 80 * 1024) {
+    // range launches on the MaxNorm codebook with 16-bit results
+    const long long tasks = (long long)((a.max_len + C4::CHUNK - 1) / C4::CHUNK) * grid.y * grid.z;
+    if (tasks > 3ll * device_cus() && a.out_dtype != kF32 && !a.cb_args) return launch_stream_c<CQ, INLINE>(a, grid, st, ap);
+  }
   if constexpr (INLINE && C::WAVES != 4) {
     const long long wgs = (long long)((a.max_len + C::CHUNK - 1) / C::CHUNK) * grid.y * grid.z;
     if (wgs > device_cus()) return launch_stream_c<C4, INLINE>(a, grid, st, ap);

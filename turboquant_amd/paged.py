@@ -53,8 +53,11 @@ def _rows(t: torch.Tensor, dtype: torch.dtype, shape, what: str, dev: int) -> Tu
 
 
 def _current() -> int:
-    """The current device; -1 without one (no tensor is there)."""
-    return _device() if torch.cuda.is_initialized() else -2
+    """The current device; -2 without one (no tensor is there)."""
+    try:
+        return _device()
+    except RuntimeError:
+        return -2
 
 
 class PagedLayer:
