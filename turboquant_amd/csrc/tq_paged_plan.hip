@@ -77,7 +77,7 @@ __device__ __forceinline__ void write_none(const PlanArgs &a, int t) {
 __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
   __shared__ int s_sum[kWaves];
   __shared__ Item s_item[kThreads];
-  __shared__ int s_items;
+  __shared__ int s_items, s_used;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int page = 1 << a.shift;
   const long long room = (long long)a.width << a.shift;
@@ -107,10 +107,11 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     released += total;
   }
   const long long avail = min(free0 + released, (long long)a.capacity);
+  if (tid == 0) s_used = 0;
   __syncthreads();  // the stack is whole before pages are taken from it
 
   // ---- the others take theirs ----
-  long long start0 = 0, taken0 = 0, used = 0;
+  long long start0 = 0, taken0 = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
     const int b = b0 + tid;
     const bool live = b < a.batch;
@@ -119,17 +120,16 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     long long total, all_need;
     const long long start = start0 + block_prefix(n, s_sum, lane, wave, total);
     start0 += total;
+    if (tid == 0) s_items = 0;  // all have passed the scan's barriers, so the round before
     const bool has_room = (long long)kv + n <= room && start + n <= a.tokens;
     const int held = pages_of(kv);
     const int need = has_room ? pages_of((long long)kv + n) - held : 0;
     const long long taken = taken0 + block_prefix(need, s_sum, lane, wave, all_need);
     taken0 += all_need;
     const bool fits = has_room && (need == 0 || taken + need <= avail);
-    long long got;
-    (void)block_prefix(fits ? need : 0, s_sum, lane, wave, got);
-    used += got;
-    if (tid == 0) s_items = 0;
-    __syncthreads();
+    // the requests that fit and need pages are the first that need any, so what
+    // is taken ends with the last of them
+    if (fits && need > 0) atomicMax(&s_used, (int)(taken + need));
     if (live) {
       a.starts[b] = (int)min(start, 0x7fffffffll);
       a.appended[b] = fits ? n : 0;
@@ -169,9 +169,10 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
       }
     }
   }
+  __syncthreads();
   if (tid == 0) {
     a.starts[a.batch] = (int)min(start0, 0x7fffffffll);
-    a.free_out[0] = (int)(avail - used);
+    a.free_out[0] = (int)(avail - s_used);
   }
   if (a.apart) return;
   for (long long t = start0 + tid; t < a.tokens; t += kThreads) write_none(a, (int)t);

@@ -3,9 +3,14 @@
 // The codec is the contiguous cache's (tq_pqo_dev.h: one lane a 32-element
 // block); what differs is where a record lies: slot s of KV head g is record
 // ((s / page_size) num_kv_heads + g) page_size + s % page_size.  Consecutive
-// lanes take the blocks of consecutive tokens of one head, so the records of
-// a run of slots are written and read as one run.  Bound by HBM for prompts
-// and by the launch for a token per request.
+// lanes take consecutive blocks of the activations, which are four to five
+// times the records' bytes; a workgroup's eight tokens (8 heads of 128) still
+// make runs of 384 bytes in each head's records.  Bound by HBM for prompts and
+// by the launch for a token per request: 8,000 tokens of 3-bit codes, 8 heads
+// of 128, are stored in 13.5 us and loaded in 11.5 (40 MB each, 3.0 and 3.5
+// TB/s), 64,000 in 80 and 53 (4.0 and 6.0 TB/s).  Lanes along the tokens of one
+// head, so that records are one run and activations pieces of a head, store
+// them in 87.
 #include "tq_paged.h"
 #include "tq_sketch_dev.h"
 
@@ -27,6 +32,14 @@ __device__ __forceinline__ long long paged_record(const Pages &p, int t, int g) 
   const long long s = p.slots[t];
   if (s < 0 || s >= p.num_slots) return -1;
   return (((s >> p.shift) * p.heads + g) << p.shift) + (s & ((1 << p.shift) - 1));
+}
+
+// Consecutive workgroups go to the eight dies in turn; this gives each die a run
+// of the work, so that a line of records that two workgroups write is whole in
+// one L2 (64,000 tokens stored in 91 us in turn, in 82 so).
+__device__ __forceinline__ int die_order(int b, int n) {
+  const int q = n >> 3;
+  return b < 8 * q ? (b & 7) * q + (b >> 3) : b;
 }
 
 // Block at element i of x, by 16-byte loads where `vec`.
@@ -61,17 +74,20 @@ struct StoreArgs {
   float cb[16], decode_factor, inv_sqrt_d;
 };
 
-// grid (blocks of tokens x blocks, heads, keys and values)
+// grid (tokens x heads x blocks, keys and values)
 template <int BITS, int CB, int DT, int NORM>
 __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
-  const int lin = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y, z = blockIdx.z;
-  const int t = lin / a.num_blocks, qb = lin - t * a.num_blocks;
-  const long long rec = paged_record(a.pages, t, g);
-  if (rec < 0) return;
+  const int lin = die_order(blockIdx.x, gridDim.x) * 256 + threadIdx.x, z = blockIdx.y;
+  const int v = lin / a.num_blocks, qb = lin - v * a.num_blocks;
+  const int t = v / a.pages.heads, g = v - t * a.pages.heads;
+  if (t >= a.pages.tokens) return;
+  // encoded whether its slot names a token or not: the block's load does not wait for the slot's
   float r[32];
   load_at<DT>(a.x[z], t * a.stride[z] + ((long long)g * a.num_blocks + qb) * 32, a.vec[z], r);
+  const long long rec = paged_record(a.pages, t, g);
   uint32_t w[BITS];
   const float s = encode_block<BITS, CB, true, NORM>(r, a.qc, w);
+  if (rec < 0) return;
   const long long blk = rec * a.num_blocks + qb;
   store_packed<BITS>(a.idx[z], blk, w);
   a.sc[z][blk] = f32_to_f16(s * a.qc.scale_sign);
@@ -128,57 +144,72 @@ struct LoadArgs {
   const uint8_t *idx[2];
   const uint16_t *sc[2];
   void *out[2];
-  int num_blocks;
+  int num_blocks, through;  // through: tqh::store16
   float cb[16], sgm;  // the centroids and the decode signs' magnitude
 };
 
 // out_j = fl(fl(W_j * fl(1/sqrt(32))) * |scale|), W = butterfly(cb[code] sign),
 // the values of tq_polar_dequantize.
+// A wave's 64 blocks are staged in LDS (rows padded by 16 bytes), so that a
+// store instruction writes 1 KB in one run instead of 16 bytes into each of 64
+// places (8,000 tokens in 17 -> 12 us).
 template <int BITS, int DT>
 __global__ __launch_bounds__(256) void paged_load_kernel(LoadArgs a) {
+  constexpr int NDW = DT == kF32 ? 32 : 16, RS = NDW + 4;  // words of a block
   __shared__ float lut[16];
+  __shared__ __attribute__((aligned(16))) uint32_t s_out[4][64 * RS];
 #pragma unroll
   for (int i = 0; i < 16; i++)
     if (threadIdx.x == i) lut[i] = a.cb[i] * a.sgm;
   __syncthreads();
-  const int lin = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y, z = blockIdx.z;
-  const int t = lin / a.num_blocks, qb = lin - t * a.num_blocks;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, z = blockIdx.y;
+  const int lin0 = blockIdx.x * 256 + 64 * wave, lin = lin0 + lane;  // blocks in the output's order
+  const int v = lin / a.num_blocks, qb = lin - v * a.num_blocks;
+  const int t = v / a.pages.heads, g = v - t * a.pages.heads;
   const long long rec = paged_record(a.pages, t, g);
-  if (rec < 0) return;
-  const long long blk = rec * a.num_blocks + qb;
-  const uint32_t *p = reinterpret_cast<const uint32_t *>(a.idx[z] + blk * (4 * BITS));
-  uint32_t w[BITS];
-  if constexpr (BITS == 4) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else {
+  const unsigned long long live = __ballot(rec >= 0);
+  uint32_t *row = s_out[wave] + lane * RS;
+  if (rec >= 0) {
+    const long long blk = rec * a.num_blocks + qb;
+    const uint32_t *p = reinterpret_cast<const uint32_t *>(a.idx[z] + blk * (4 * BITS));
+    uint32_t w[BITS];
+    if constexpr (BITS == 4) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(p);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < BITS; i++) w[i] = p[i];
+      for (int i = 0; i < BITS; i++) w[i] = p[i];
+    }
+    const float s = fabsf(f16_to_f32(a.sc[z][blk]));
+    float y[32];
+#pragma unroll
+    for (int j = 0; j < 32; j++) {
+      const float c = lut[field<BITS>(w, j)];
+      y[j] = pqo_neg(j) ? -c : c;
+    }
+    butterfly<32>(y);
+#pragma unroll
+    for (int j = 0; j < 32; j++) y[j] = (y[j] * kInvSqrt32) * s;
+    uint32_t o[NDW];
+#pragma unroll
+    for (int j = 0; j < NDW; j++) {
+      if constexpr (DT == kF32) o[j] = f2u(y[j]);
+      else if constexpr (DT == kBF16) o[j] = pack_bf16x2(y[2 * j], y[2 * j + 1]);
+      else o[j] = (uint32_t)f32_to_f16(y[2 * j]) | ((uint32_t)f32_to_f16(y[2 * j + 1]) << 16);
+    }
+#pragma unroll
+    for (int j = 0; j < NDW / 4; j++)
+      *reinterpret_cast<uint4 *>(row + 4 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
   }
-  const float s = fabsf(f16_to_f32(a.sc[z][blk]));
-  float y[32];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  uint32_t *const out = static_cast<uint32_t *>(a.out[z]) + (long long)lin0 * NDW;
 #pragma unroll
-  for (int j = 0; j < 32; j++) {
-    const float c = lut[field<BITS>(w, j)];
-    y[j] = pqo_neg(j) ? -c : c;
-  }
-  butterfly<32>(y);
-#pragma unroll
-  for (int j = 0; j < 32; j++) y[j] = (y[j] * kInvSqrt32) * s;
-  const long long e = (((long long)t * a.pages.heads + g) * a.num_blocks + qb) * 32;
-  if constexpr (DT == kF32) {
-    float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(a.out[z]) + e);
-#pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
-  } else {
-    uint32_t v[16];
-#pragma unroll
-    for (int j = 0; j < 16; j++)
-      v[j] = DT == kBF16 ? pack_bf16x2(y[2 * j], y[2 * j + 1])
-                         : (uint32_t)f32_to_f16(y[2 * j]) | ((uint32_t)f32_to_f16(y[2 * j + 1]) << 16);
-    uint4 *o = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out[z]) + e);
-#pragma unroll
-    for (int j = 0; j < 4; j++) o[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  for (int q = 0; q < NDW / 4; q++) {
+    const int f = 256 * q + 4 * lane, r = f / NDW, c = f % NDW;  // block r of the wave, its words c .. c + 3
+    if ((live >> r) & 1)
+      tqh::store16(out + f, *reinterpret_cast<const tqh::words4 *>(s_out[wave] + r * RS + c), a.through);
   }
 }
 
@@ -225,7 +256,7 @@ extern "C" int tq_paged_store(const void *k, long long k_stride, const void *v, 
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "null pointer");
   if (!aligned16(k_indices) || !aligned16(v_indices) || !aligned16(k_scales) || !aligned16(v_scales))
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "code and scale pools start on 16-byte boundaries");
-  const long long lanes = (long long)tokens * (head_dim / 32);
+  const long long lanes = (long long)tokens * num_kv_heads * (head_dim / 32);
   if (lanes >= 1ll << 30) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "too many tokens in one call");
   const int size = tqh::dtype_size(dtype);
   a.pages.slots = slots;
@@ -269,7 +300,7 @@ extern "C" int tq_paged_store(const void *k, long long k_stride, const void *v, 
     });
     return tqh::check_launch("paged_store_tq_kernel");
   }
-  const dim3 grid((unsigned)((lanes + 255) / 256), (unsigned)num_kv_heads, 2);
+  const dim3 grid((unsigned)((lanes + 255) / 256), 2);
   by_type(dtype, [&](auto dt) {
     auto go = [&](auto b, auto c) {
       constexpr int B = decltype(b)::value, C = decltype(c)::value, DT = decltype(dt)::value;
@@ -304,7 +335,7 @@ extern "C" int tq_paged_load(const uint8_t *k_indices, const uint16_t *k_scales,
   if (!aligned16(k_indices) || !aligned16(v_indices) || !aligned16(k_scales) || !aligned16(v_scales) ||
       !aligned16(k_out) || !aligned16(v_out))
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "pools and outputs start on 16-byte boundaries");
-  const long long lanes = (long long)tokens * (head_dim / 32);
+  const long long lanes = (long long)tokens * num_kv_heads * (head_dim / 32);
   if (lanes >= 1ll << 30) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "too many tokens in one call");
   a.pages.slots = slots;
   a.pages.num_slots = num_pages << a.pages.shift;
@@ -317,9 +348,10 @@ extern "C" int tq_paged_load(const uint8_t *k_indices, const uint16_t *k_scales,
   a.out[0] = k_out;
   a.out[1] = v_out;
   a.num_blocks = head_dim / 32;
+  a.through = 2 * lanes * 32 * tqh::dtype_size(out_dtype) > tqh::kThroughBytes;
   for (int i = 0; i < codec.cb.nc; i++) a.cb[i] = codec.cb.c[i];
   a.sgm = decode_factor();
-  const dim3 grid((unsigned)((lanes + 255) / 256), (unsigned)num_kv_heads, 2);
+  const dim3 grid((unsigned)((lanes + 255) / 256), 2);
   by_type(out_dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (bits == 3) hipLaunchKernelGGL((paged_load_kernel<3, DT>), grid, dim3(256), 0, stream, a);
