@@ -41,6 +41,13 @@ def _ptr(t: torch.Tensor, dtype: torch.dtype, shape, what: str, dev: int) -> int
     _refuse(t, dtype, shape, what)
 
 
+def _addr(t: torch.Tensor, dtype: torch.dtype, what: str, dev: int) -> int:
+    """The same for a tensor whose shape is right already."""
+    if t.dtype is dtype and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(t, dtype, t.shape, what)
+
+
 def _rows(t: torch.Tensor, dtype: torch.dtype, shape, what: str, dev: int) -> Tuple[int, int]:
     """Address and row stride (elements) of t [tokens, heads, head_dim], heads adjacent, likewise."""
     n, h, d = shape
@@ -144,15 +151,15 @@ def paged_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     and its pages go back), block_table int32 [batch, width] and free_pages
     int32 [capacity] (written), free_count int32 [1].  kv_lens_out and
     free_count_out may be the inputs; new tensors by default."""
-    if kv_lens.dim() != 1 or block_table.dim() != 2 or free_pages.dim() != 1:
+    lens, table, pages, i32, dev = kv_lens.shape, block_table.shape, free_pages.shape, torch.int32, _current()
+    if len(lens) != 1 or len(table) != 2 or len(pages) != 1 or table[0] != lens[0]:
         raise ValueError("kv_lens [batch], block_table [batch, width] and free_pages [capacity] are expected")
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
-    lens, i32, dev = kv_lens.shape, torch.int32, _current()
-    b, width, cap = lens[0], block_table.shape[1], free_pages.shape[0]
-    ins = (_ptr(kv_lens, i32, lens, "kv_lens", dev), _ptr(new_lens, i32, lens, "new_lens", dev), b,
-           _ptr(block_table, i32, (b, width), "block_table", dev), width,
-           _ptr(free_pages, i32, (cap,), "free_pages", dev), cap, _ptr(free_count, i32, (1,), "free_count", dev))
+    b = lens[0]
+    ins = (_addr(kv_lens, i32, "kv_lens", dev), _ptr(new_lens, i32, lens, "new_lens", dev), b,
+           _addr(block_table, i32, "block_table", dev), table[1], _addr(free_pages, i32, "free_pages", dev), pages[0],
+           _ptr(free_count, i32, (1,), "free_count", dev))
     slots = kv_lens.new_empty(num_tokens, dtype=torch.int64)
     rows = kv_lens.new_empty(num_tokens + 2 * b + 1)
     first = rows.data_ptr()
@@ -190,11 +197,13 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
         qo, ko = out
         qop, qo0 = _rows(qo, dt, qs, "out[0]", dev)
         kop, ko0 = _rows(ko, dt, ks, "out[1]", dev)
-    half = inv_freq.numel()
+    half = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
+    if half < 0:
+        raise ValueError("inv_freq must be [rot_dim / 2]")
     wq = None if q_weight is None else _ptr(q_weight, dt, (d,), "q_weight", dev)
     wk = None if k_weight is None else _ptr(k_weight, dt, (d,), "k_weight", dev)
     check(lib.tq_qk_norm_rope(qp, q0, kp, k0, _DT[dt], _ptr(positions, torch.int32, (t,), "positions", dev), t, h, hk,
-                              d, _ptr(inv_freq, torch.float32, (half,), "inv_freq", dev), 2 * half,
+                              d, _addr(inv_freq, torch.float32, "inv_freq", dev), 2 * half,
                               1 if interleaved else 0, wq, wk, eps, qop, qo0, kop, ko0, _stream()))
     return qo, ko
 
@@ -207,12 +216,13 @@ def paged_store(layer: PagedLayer, slots: torch.Tensor, k: torch.Tensor, v: torc
     pages are skipped, the others' slots are distinct.  sign_matrix: TQ records,
     whose keys are sketched too."""
     t, hk, d, dt, dev = slots.shape[0], layer.num_kv_heads, layer.head_dim, k.dtype, _current()
-    if dt not in _DT or k.dim() != 3 or v.dim() != 3:
-        raise ValueError("k and v [tokens, num_kv_heads, head_dim] must be f32/bf16/f16")
+    if dt not in _DT or k.dim() != 3 or v.dim() != 3 or slots.dim() != 1:
+        raise ValueError("slots [tokens], k and v [tokens, num_kv_heads, head_dim] (f32/bf16/f16) are expected")
     sg, nm, rm = layer._check(bits, sign_matrix, dev)
-    kp, k0 = _rows(k, dt, (t, hk, d), "k", dev)
-    vp, v0 = _rows(v, dt, (t, hk, d), "v", dev)
-    check(lib.tq_paged_store(kp, k0, vp, v0, _DT[dt], _ptr(slots, torch.int64, (t,), "slots", dev), t, *layer._ptrs,
+    shape = (t, hk, d)
+    kp, k0 = _rows(k, dt, shape, "k", dev)
+    vp, v0 = _rows(v, dt, shape, "v", dev)
+    check(lib.tq_paged_store(kp, k0, vp, v0, _DT[dt], _addr(slots, torch.int64, "slots", dev), t, *layer._ptrs,
                              sg, nm, rm, layer.num_pages, hk, layer.page_size, d, bits, outlier_blocks, norm_mode,
                              _stream()))
 
@@ -224,6 +234,8 @@ def paged_load(layer: PagedLayer, slots: torch.Tensor, bits: int, outlier_blocks
     num_kv_heads, head_dim] in out_dtype, or into `out`; rows whose slot is
     outside the pages are left as they are."""
     shape, dev = (slots.shape[0], layer.num_kv_heads, layer.head_dim), _current()
+    if slots.dim() != 1:
+        raise ValueError("slots [tokens] are expected")
     layer._check(bits, None, dev)
     if out is None:
         out = slots.new_empty(shape, dtype=out_dtype), slots.new_empty(shape, dtype=out_dtype)
@@ -231,7 +243,7 @@ def paged_load(layer: PagedLayer, slots: torch.Tensor, bits: int, outlier_blocks
     dt = k.dtype
     if dt not in _DT:
         raise ValueError("out must be f32/bf16/f16")
-    check(lib.tq_paged_load(*layer._ptrs, _ptr(slots, torch.int64, shape[:1], "slots", dev), shape[0], layer.num_pages,
+    check(lib.tq_paged_load(*layer._ptrs, _addr(slots, torch.int64, "slots", dev), shape[0], layer.num_pages,
                             shape[1], layer.page_size, shape[2], bits, outlier_blocks, norm_mode,
                             _ptr(k, dt, shape, "out[0]", dev), _ptr(v, dt, shape, "out[1]", dev), _DT[dt], _stream()))
     return k, v
@@ -249,21 +261,23 @@ def paged_decode_attention(q: torch.Tensor, layer: PagedLayer, block_table: torc
     this batch, heads and max_kv_len; one call at a time uses it.  Returns
     [batch, heads, head_dim] in out_dtype (q's by default)."""
     shape, dt, dev = q.shape, q.dtype, _current()
-    if len(shape) != 3 or shape[2] != layer.head_dim or block_table.dim() != 2:
+    table = block_table.shape
+    if len(shape) != 3 or shape[2] != layer.head_dim or len(table) != 2 or table[0] != shape[0]:
         raise ValueError(f"q [batch, heads, {layer.head_dim}] and block_table [batch, width] are expected")
-    (b, h, d), width = shape, block_table.shape[1]
+    b, h, d = shape
     if out is None:
         out = torch.empty_like(q) if out_dtype is None or out_dtype is dt else torch.empty_like(q, dtype=out_dtype)
-    odt = out.dtype
+    elif out.shape != shape:
+        raise ValueError(f"out must be {list(shape)}, got {list(out.shape)}")
+    odt, ws = out.dtype, workspace.buf
     if dt not in _DT or odt not in _DT:
         raise ValueError("q and out must be f32/bf16/f16")
     sg, nm, rm = layer._check(bits, sign_matrix, dev)
     check(lib.tq_paged_decode_attention(
-        _ptr(q, dt, shape, "q", dev), _DT[dt], *layer._ptrs, sg, nm, rm,
-        _ptr(block_table, torch.int32, (b, width), "block_table", dev), width,
-        _ptr(kv_lens, torch.int32, (b,), "kv_lens", dev), b, h, layer.num_kv_heads, d, bits, outlier_blocks, norm_mode,
-        layer.page_size, layer.num_pages, max_kv_len, softmax_scale, _ptr(out, odt, shape, "out", dev), _DT[odt],
-        _ptr(workspace.buf, torch.uint8, (workspace.nbytes,), "workspace", dev), workspace.nbytes, _stream()))
+        _addr(q, dt, "q", dev), _DT[dt], *layer._ptrs, sg, nm, rm, _addr(block_table, torch.int32, "block_table", dev),
+        table[1], _ptr(kv_lens, torch.int32, (b,), "kv_lens", dev), b, h, layer.num_kv_heads, d, bits, outlier_blocks,
+        norm_mode, layer.page_size, layer.num_pages, max_kv_len, softmax_scale, _addr(out, odt, "out", dev), _DT[odt],
+        _addr(ws, torch.uint8, "workspace", dev), workspace.nbytes, _stream()))
     return out
 
 
