@@ -128,6 +128,9 @@ def test_plan_lengths_out_of_range(tq):
     assert p.appended.tolist() == [3, 0, 0] and p.kv_lens.tolist() == [3, 33, 32] and p.free_count.tolist() == [3]
     assert p.slots.tolist() == [9 * 16, 9 * 16 + 1, 9 * 16 + 2, -1, -1, -1, -1, -1]
     assert p.positions.tolist() == [0, 1, 2, -1, -1, -1, -1, -1] and table.tolist()[0] == [9, 1]
+    n = 1 << 24  # the most that a step holds
+    p = tq.paged_plan(i32(0), i32(n + 9), dev(np.zeros((1, 4), np.int32)), free, i32(4), 16, n)
+    assert p.appended.tolist() == [0] and int(p.slots.max()) == -1
     p = tq.paged_plan(i32(0), i32((1 << 24) + 9), dev(np.zeros((1, 4), np.int32)), free, i32(4), 16, 4)
     assert p.appended.tolist() == [0] and p.slots.tolist() == [-1] * 4 and p.free_count.tolist() == [4]
 
@@ -272,6 +275,12 @@ def test_wrappers_refuse(tq):
                  lambda: tq.paged_plan(pos, pos, table, pos, pos[:1], 16, -1)):
         with pytest.raises(ValueError):
             call()
+    cache = tq.PagedCache(tq.CacheConfig(3, 64, 2, 1), 4, 3, 32, 16)
+    plan = cache.plan(i32(1, 1, 1), 3)
+    for call in (lambda: cache.step(0, plan, q[:2], k, k, 1.0), lambda: cache.step(0, plan, q[:0], k[:0], k[:0], 1.0),
+                 lambda: cache.attend(0, q[:2], 1.0)):
+        with pytest.raises(ValueError):
+            call()
     with pytest.raises(tq.TurboQuantError, match="exceeds a table row"):
         tq.paged_decode_attention(q, layer, table, pos, 3, 33, 1.0, ws)
 
@@ -403,11 +412,13 @@ def sign_rows(rmat, d):
     return 1.0 - 2.0 * ((w[:, :, None] >> np.arange(32)) & 1).reshape(d, d)
 
 
-def attend(q, recs, scale, rmat, skip=None):
+def attend(q, recs, scale, rmat, skip=None, codebook=0.0):
     """64-bit attention of q [H, D] over a request's records, and a bound of a kernel's error: logits of two-part f16
     operands are off by 2^-20 of the sum of their terms' sizes (twice that where a correction joins), weights by as
     much twice (numerator and sum), and values, whose products are cut likewise and whose offset grows them by up to
-    2 x 2.16 x sqrt(32), by 2^-16 of the largest."""
+    2 x 2.16 x sqrt(32), by 2^-16 of the largest.  `codebook`: centroids off by as much of their size, so logits by as
+    much of their terms', and a value, 32 centroids in an orthogonal transform, by sqrt(32) times as much of the
+    largest."""
     h, d = q.shape
     out, bound = np.zeros((h, d)), np.zeros((h, 1))
     if recs is None:
@@ -427,7 +438,7 @@ def attend(q, recs, scale, rmat, skip=None):
         w = np.exp((x - x.max()) * scale)
         out[i] = w @ v[:, g] / w.sum()
         top = np.abs(v[:, g]).max()
-        bound[i] = top * (4 * scale * 2.0 ** -20 * size.max() + 2.0 ** -16)
+        bound[i] = top * (4 * scale * (2.0 ** -20 + codebook) * size.max() + 2.0 ** -16 + codebook * math.sqrt(32))
     return out, bound
 
 
@@ -443,8 +454,10 @@ def check_attention(tq, lens, page, width, hq, hk, d, bits, mode, dtype="bf16", 
     ws = tq.AttentionWorkspace(len(lens), hq, hk, d, most)
     got = tq.paged_decode_attention(q, layer, table, i32(*lens), bits, most, d ** -0.5, ws, ob, sign_matrix=rmat,
                                     out_dtype=DT[out])
+    # 16-bit results of 3-bit codes may come from a codebook rounded to f16 at its best scale
+    codebook = 2.0 ** -15.4 if bits == 3 and out != "f32" else 0.0
     for b in range(len(lens)):
-        ref, bound = attend(as64(q[b]), recs[b], d ** -0.5, rmat)
+        ref, bound = attend(as64(q[b]), recs[b], d ** -0.5, rmat, codebook=codebook)
         err = np.abs(as64(got[b]) - ref)
         assert (err <= bound + half_step(ref, out)).all(), (b, lens[b], float(err.max()), float(bound.max()))
     return q, layer, table, ob, rmat, recs, ws
@@ -477,19 +490,34 @@ def test_decode_types(tq, dtype, out, mode, bits):
     check_attention(tq, [90, 1300], 64, 21, 8, 2, 128, bits, mode, dtype, out)
 
 
-@pytest.mark.parametrize("mode,bits", [("pqo", 3), ("pqo", 4), ("pq", 4), ("tq", 3)])
-def test_decode_long(tq, mode, bits):
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("mode,bits", [("pqo", 3), ("pqo", 4), ("pq", 3), ("pq", 4), ("tq", 3), ("tq", 4)])
+def test_decode_long(tq, mode, bits, out):
     """Contexts split over many workgroups, joined, beside short ones."""
-    check_attention(tq, [20001, 37, 9000], 64, 320, 4, 2, 128, bits, mode)
+    check_attention(tq, [20001, 37, 9000], 64, 320, 4, 2, 128, bits, mode, out=out)
 
 
-@pytest.mark.parametrize("batch,hk", [(70, 8), (200, 2), (300, 1), (64, 16), (40, 40)])
-def test_decode_many_requests(tq, batch, hk):
-    """More (request, KV head) pairs than workgroups are resident at once, some of them empty."""
+@pytest.mark.parametrize("batch,hk,group,out", [(70, 8, 1, "f32"), (200, 2, 1, "bf16"), (300, 1, 1, "f32"),
+                                                (300, 1, 2, "f16"), (64, 16, 1, "f16"), (40, 40, 1, "f32"),
+                                                (64, 8, 4, "f16"), (90, 8, 2, "bf16"), (20, 40, 1, "f16"),
+                                                (40, 4, 16, "f16"), (256, 4, 1, "f16"), (257, 4, 1, "f16")])
+@pytest.mark.parametrize("mode,bits", [("pqo", 3), ("pqo", 4), ("tq", 3)])
+def test_decode_many_requests(tq, batch, hk, group, out, mode, bits):
+    """About and more (request, KV head) pairs than workgroups are resident at once, some of them empty."""
     rng = np.random.default_rng(batch)
     lens = rng.integers(0, 900, size=batch).tolist()
     lens[3], lens[-1] = 0, 1800
-    check_attention(tq, lens, 64, 29, hk, hk, 64, 3, "pqo")
+    check_attention(tq, lens, 64, 29, hk * group, hk, 64, bits, mode, out=out)
+
+
+@pytest.mark.parametrize("d,group", [(32, 1), (32, 8), (128, 1), (128, 4), (128, 8), (256, 2), (256, 8)])
+@pytest.mark.parametrize("mode,bits", [("pqo", 3), ("pq", 3), ("tq", 3), ("pqo", 4)])
+def test_decode_range_launches(tq, d, group, mode, bits):
+    """16-bit results of batches that take ranges of several chunks, at every shape of head; pages from tile to chunk."""
+    if mode == "tq" and d == 32:
+        pytest.skip("no sketch of 32 elements")
+    lens = [5000, 1, 128, 127, 129, 513, 2047, 4096, 0, 3333, 511, 1025] * 2
+    check_attention(tq, lens, 16 if group == 1 else 256, 320 if group == 1 else 20, 8 * group, 8, d, bits, mode, out="f16")
 
 
 def test_decode_lengths_are_clamped(tq):

@@ -464,10 +464,7 @@ extern "C" int tq_paged_decode_attention(const void *q, int q_dtype, const uint8
   a.qjl_signs = reinterpret_cast<const uint32_t *>(signs);
   a.qjl_norms = norms;
   a.qjl_c = tq_qjl_bias_scale(head_dim);
-  // The passes that contract 4-bit codes before their offset is taken off lose
-  // up to 1e-3 of a long context's small outputs: a bf16 result's own rounding
-  // is larger, f16 and f32 results take the codebook.
-  if (codec.norm_mode == TQ_NORM_L2NORM || (bits == 4 && out_dtype != TQ_DTYPE_BF16)) {
+  if (codec.norm_mode == TQ_NORM_L2NORM) {
     a.cb_args = 1;
     for (int i = 0; i < codec.cb.nc; i++) a.cb[i] = codec.cb.c[i];
   }

@@ -98,6 +98,16 @@ __device__ __forceinline__ u32x4 nib_operand(uint32_t w) {
   const uint32_t h = w >> 8;
   return u32x4{w & 0x000F000Fu, w & 0x00F000F0u, h & 0x000F000Fu, h & 0x00F000F0u};
 }
+// The same codes, in the same places, as 1 + i / 16: normal numbers, whose
+// products keep their 22 bits (with a subnormal operand the matrix cores align
+// a product as if its leading zeros were there: i 2^-24 keeps ten bits fewer,
+// and long contexts' outputs end 1.5e-3 off; so, 4e-6).  Three instructions
+// more an operand: 16 sequences of up to 16,384 tokens, 32 over 8 heads, 48.3 ->
+// 53.0 us, where the codebook's pairs, as exact, take 63.4.
+__device__ __forceinline__ u32x4 nib_normal(uint32_t w) {
+  constexpr uint32_t M = 0x03C003C0u, ONE = 0x3C003C00u;
+  return u32x4{((w << 6) & M) | ONE, ((w << 2) & M) | ONE, ((w >> 2) & M) | ONE, ((w >> 6) & M) | ONE};
+}
 
 // Read p's CODES BITS-bit codes of a lane's stream w (little-endian words), as
 // the byte offset of their table entry (codes * 8): two VALU each.
@@ -286,6 +296,8 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
   // the product: no codebook reads, half the instructions of the two-part
   // codebook operand.
   static_assert(!GRID || (BITS == 4 && C::MODE == kModePqo), "the grid passes take 4-bit PQO codes");
+  // Over pages the codes are normal numbers (nib_normal).
+  constexpr bool NORMAL = GRID && PAGED;
   constexpr int KJA = GRID ? QPM : KJ;                  // key-pass instructions per qblock group
   constexpr bool QAR = GRID || C::QA_REGS;              // query operands in registers
   __shared__ __attribute__((aligned(16))) float lds[C::TOTAL - LSH];
@@ -950,7 +962,7 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
       const float4 lo4 = *reinterpret_cast<const float4 *>(src), hi4 = *reinterpret_cast<const float4 *>(src + 4);
       // registers 0 and 2 meet codes i 2^-24, 1 and 3 codes i 2^-20
       // (nib_operand): the former take the factor 16 (exact)
-      const float sc16 = sc * 16.f;
+      const float sc16 = NORMAL ? sc : sc * 16.f;
       const float xa[4] = {lo4.x * sc16, lo4.y * sc, lo4.z * sc16, lo4.w * sc};
       const float xb[4] = {hi4.x * sc16, hi4.y * sc, hi4.z * sc16, hi4.w * sc};
       uint32_t w[4];
@@ -982,15 +994,17 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
   // hl0 + u; their R sum_j Q_j (Q as in the operand, exact power-of-two scale)
   float rqs[GRID ? QG : 1][2];
   constexpr float kGridR = 2.1573f;                       // -c_0 of the 4-bit MaxNorm codebook
-  constexpr float kGridD20 = ((2.0f * kGridR) / 15.0f) * 1048576.0f;  // D 2^20 (products enter as x i 2^-20)
-  constexpr float kGridR20 = kGridR * 1048576.0f;                     // R 2^20
+  // D 2^20 and R 2^20 (products enter as x i 2^-20); NORMAL: x (1 + i / 16) enters
+  constexpr float kGridD = (2.0f * kGridR) / 15.0f;
+  constexpr float kGridD20 = NORMAL ? kGridD * 16.0f : kGridD * 1048576.0f;
+  constexpr float kGridR20 = NORMAL ? kGridR + kGridD * 16.0f : kGridR * 1048576.0f;
   if constexpr (GRID) {
 #pragma unroll
     for (int qg = 0; qg < QG; qg++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int hl = min(hl0 + u, HG - 1);
-        rqs[qg][u] = kGridR * s_qsum[hl * NQB + qg * QPM + lg / ES] * exp2i(-head_exp(s_qmax, hl));
+        rqs[qg][u] = (NORMAL ? kGridR20 : kGridR) * s_qsum[hl * NQB + qg * QPM + lg / ES] * exp2i(-head_exp(s_qmax, hl));
       }
   }
   float escale[NS], erscale[NS];
@@ -1093,7 +1107,7 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
       for (int qg = 0; qg < QG; qg++)
 #pragma unroll
         for (int j = 0; j < KJA; j++) {
-          dk[qg] = mfma(qa[qg * KJA + j], nib_operand(kw[i][qg][j]), dk[qg]);
+          dk[qg] = mfma(qa[qg * KJA + j], NORMAL ? nib_normal(kw[i][qg][j]) : nib_operand(kw[i][qg][j]), dk[qg]);
         }
     } else {
     // every pair-table read of the tile goes out before its first MFMA, so
@@ -1208,7 +1222,7 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
 #pragma unroll
     for (int qb = 0; qb < NQB; qb++) {
       // the grid V pass: even tokens' weights meet codes i 2^-24 (nib_operand), so they take the factor 16
-      const float f = GRID && ((C::TPL * lane + u) & 1) == 0 ? vinv * 16.f : vinv;
+      const float f = GRID && !NORMAL && ((C::TPL * lane + u) & 1) == 0 ? vinv * 16.f : vinv;
       st_s[qb * C::PSTR + C::TPL * lane + u] = svv[u][qb] * f;
     }
   if (MULTI && l16 == 0) {
@@ -1295,10 +1309,10 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
       for (int j = 0; j < GC; j++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          acc[vs * GC + j] = mfma(nib_operand(cw[j][h]), bw[h], acc[vs * GC + j]);
+          acc[vs * GC + j] = mfma(NORMAL ? nib_normal(cw[j][h]) : nib_operand(cw[j][h]), bw[h], acc[vs * GC + j]);
         }
-      // a code of 1 in nib_operand's scales: 2^-24 in registers 0 and 2, 2^-20 in 1 and 3
-      constexpr uint32_t kOne = 0x00010001u, kOne16 = 0x00100010u;
+      // a code of 1 in nib_operand's scales: 2^-24 in registers 0 and 2, 2^-20 in 1 and 3 (NORMAL: 1)
+      constexpr uint32_t kOne = NORMAL ? 0x3C003C00u : 0x00010001u, kOne16 = NORMAL ? kOne : 0x00100010u;
 #pragma unroll
       for (int h = 0; h < 2; h++) acc1[vs] = mfma(u32x4{kOne, kOne16, kOne, kOne16}, bw[h], acc1[vs]);
     }

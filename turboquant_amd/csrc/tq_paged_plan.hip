@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     const int b = b0 + tid;
     const bool live = b < a.batch;
     const int kv = live ? kv_of(b) : 0, raw = live ? a.new_lens[b] : 0;
-    const int n = min(max(raw, 0), kMaxTokens);
+    const int n = min(max(raw, 0), kMaxTokens + 1);  // one more than any step holds: it does not fit
     long long total, all_need;
     const long long start = start0 + block_prefix(n, s_sum, lane, wave, total);
     start0 += total;

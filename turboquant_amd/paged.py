@@ -360,12 +360,15 @@ class PagedCache:
              softmax_scale: float, rope: Optional[QkNormRope] = None) -> torch.Tensor:
         """A decode step of a layer: norm and rotation of q and k [num_tokens,
         heads, head_dim], the new records, and the attention of each request's
-        last token: [max_requests, heads, head_dim].  Rows of requests that
-        bring no token in this step hold nothing of use."""
+        last token: [max_requests, heads, head_dim].  Rows of requests to which
+        the plan appended nothing hold nothing of use."""
+        if q.dim() != 3 or q.shape[0] == 0 or q.shape[0] != plan.slots.shape[0]:
+            raise ValueError(f"q must be [{plan.slots.shape[0]}, heads, head_dim], a row for each of the plan's tokens "
+                             "(at least one)")
         if rope is not None:
             q, k = qk_norm_rope(q, k, plan.positions, *rope)
         self.store(layer, plan, k, v)
-        rows = (plan.starts[1:] - 1).clamp_(0, max(q.shape[0] - 1, 0))
+        rows = (plan.starts[1:] - 1).clamp_(0, q.shape[0] - 1)
         return self.attend(layer, q.index_select(0, rows), softmax_scale)
 
     def memory_usage(self) -> int:
