@@ -7,7 +7,11 @@
 // wave, the waves' totals through LDS) and carries the sums on, so the free
 // list, which every sum goes by, is read and written in order and the step
 // needs one launch.  The launch and three dependent reads (lengths, free
-// count, pages) bound it.
+// count, pages) bound it: 64 decoding requests take 6.3 us.  The rows of a step
+// of more than kApart tokens are a second launch's, a lane a token: 512 requests
+// with 87,552 rows take 13.5 + 4.0 us, in one workgroup 36.  (Up to 4,096 rows
+// the second launch costs more than it saves: 2,131 rows 12.6 us a call, 4,198
+// rows 14.7.)
 #include "tq_mfma.h"
 #include "tq_paged.h"
 
@@ -17,10 +21,7 @@ using namespace tqm;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kMaxTokens = 1 << 24, kMaxWidth = 1 << 20;
-#ifndef TQ_PLAN_APART
-#define TQ_PLAN_APART 4096
-#endif
-constexpr int kApart = TQ_PLAN_APART;  // steps of more tokens: their rows by a launch of their own
+constexpr int kApart = 4096;  // steps of more tokens: their rows by a launch of their own
 // A request with at most this many new pages and tokens is written by its own
 // lane, a larger one by a wave.
 constexpr int kLaneItems = 2;
@@ -55,7 +56,7 @@ __device__ __forceinline__ long long block_prefix(int v, int *s, int lane, int w
 // What a request of the current 1,024 has to write.
 struct Item {
   int b, held, need, kv, n, start;
-  long long top;  // stack index of its first new page
+  long long top;  // stack index of its first new page, or of the first that it gives back
 };
 
 __device__ __forceinline__ void write_page(const PlanArgs &a, const Item &it, int j) {
@@ -92,17 +93,26 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     const bool done = b < a.batch && a.new_lens[b] < 0;
     const int back = done ? pages_of(kv_of(b)) : 0;
     if (!__syncthreads_or(back)) continue;
+    if (tid == 0) s_items = 0;  // the barrier above: the round before has been read
     long long total;
     const long long at = free0 + released + block_prefix(back, s_sum, lane, wave, total);
-    // a wave copies its done requests' pages one request after the other
-    for (unsigned long long m = __ballot(back > 0); m; m &= m - 1) {
-      const int l = __builtin_ctzll(m);
-      const int cnt = __builtin_amdgcn_readlane(back, l);
-      const long long to = ((long long)__builtin_amdgcn_readlane((int)(at >> 32), l) << 32) |
-                           (uint32_t)__builtin_amdgcn_readlane((int)at, l);
-      const int *row = a.table + (long long)(b0 + 64 * wave + l) * a.width;
-      for (int j = lane; j < cnt; j += 64)
-        if (to + j < a.capacity) a.free_pages[to + j] = row[j];
+    if (back) s_item[atomicAdd(&s_items, 1)] = Item{b, 0, back, 0, 0, 0, at};
+    __syncthreads();
+    // a wave a request, 256 pages' reads side by side
+    const int items = s_items;
+    for (int k = wave; k < items; k += kWaves) {
+      const Item it = s_item[k];
+      const int *row = a.table + (long long)it.b * a.width;
+      for (int j0 = lane; j0 < it.need; j0 += 256) {
+        int page[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) page[u] = j0 + 64 * u < it.need ? row[j0 + 64 * u] : 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int j = j0 + 64 * u;
+          if (j < it.need && it.top + j < a.capacity) a.free_pages[it.top + j] = page[u];
+        }
+      }
     }
     released += total;
   }
