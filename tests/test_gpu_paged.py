@@ -251,6 +251,20 @@ def test_rope_zeros_infinities_and_nan(tq):
     assert qo[1, 0].isnan().any() and qo[2, 1].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d,rot", [(64, 32), (128, 6), (96, 64), (64, 0)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_rope_passes_the_rest_of_a_head_through(tq, d, rot, inter, dtype):
+    """Without a norm the elements past rot_dim come out as they are, infinities and what stands beside them too."""
+    rng = np.random.default_rng(d + rot)
+    q = heads(rng, 5, 3, d, dtype)
+    q[:, 0, rot], q[:, 1, d - 1], q[2, 2, rot + 5] = float("inf"), float("-inf"), float("inf")
+    freq = dev((10000.0 ** (-np.arange(rot // 2) / max(1, rot // 2))).astype(np.float32))
+    qo, ko = tq.qk_norm_rope(q, q[:, :2], i32(0, 1, 7, 500, 30000), freq, interleaved=inter)
+    assert torch.equal(qo[..., rot:], q[..., rot:]) and torch.equal(ko, qo[:, :2])
+    assert qo[..., :rot].isfinite().all()
+
+
 def test_wrappers_refuse(tq):
     """Shapes, types, strides and places that the wrappers check themselves."""
     q, k, pos, f = torch.zeros(3, 4, 64).cuda(), torch.zeros(3, 2, 64).cuda(), i32(0, 1, 2), torch.ones(32).cuda()

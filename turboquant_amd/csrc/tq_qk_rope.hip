@@ -208,9 +208,11 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
       float y[8];
       if constexpr (PARTNER == kNeighbour) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          y[2 * j] = x[u][2 * j] * c[j] - x[u][2 * j + 1] * s[j];
-          y[2 * j + 1] = x[u][2 * j + 1] * c[j] + x[u][2 * j] * s[j];
+        for (int j = 0; j < 4; j++) {  // past rot a neighbour has no part, an infinite one neither
+          const bool on = e0 + 2 * j < a.rot;
+          const float x0 = x[u][2 * j], x1 = x[u][2 * j + 1];
+          y[2 * j] = x0 * c[j] - (on ? x1 : 0.f) * s[j];
+          y[2 * j + 1] = x1 * c[j] + (on ? x0 : 0.f) * s[j];
         }
       } else if constexpr (PARTNER == kHalfRow) {
 #pragma unroll
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           const int e = e0 + j, o = e >= a.rot ? e : (e < a.half ? e + a.half : e - a.half);
-          y[j] = x[u][j] * c[j] + mine[o] * s[j];
+          y[j] = x[u][j] * c[j] + (e >= a.rot ? 0.f : mine[o]) * s[j];
         }
       }
       if (in && h < a.heads[which])
