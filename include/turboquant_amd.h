@@ -526,7 +526,8 @@ int tq_pqo_cache_buffers(void *cache, int layer, uint8_t **k_indices, uint16_t *
  * block_table [batch][table_width] names request b's pages in order: token t
  * sits at offset t % page_size of page block_table[b][t / page_size].  A slot
  * is page * page_size + offset; a slot outside [0, num_pages * page_size), -1
- * above all, names no token.  Code and scale pools on 16-byte boundaries.
+ * above all, names no token.  Code, scale and sign pools, and tq_paged_load's outputs, on
+ * 16-byte boundaries.
  * ========================================================================= */
 
 /* Pages, slots and positions of one step's tokens from the requests' lengths,
@@ -534,7 +535,8 @@ int tq_pqo_cache_buffers(void *cache, int layer, uint8_t **k_indices, uint16_t *
  *   kv_lens [batch]: tokens that each request holds; new_lens [batch]: tokens
  *   that it appends, 0 for none, negative: it is done, and its pages go back.
  *   free_pages [free_capacity]: the free pages are entries 0 .. *free_count -
- *   1, taken from the end; pages of done requests are put there first.
+ *   1, taken from the end; pages of done requests are put there first (what
+ *   passes free_capacity is lost: one entry per page is enough).
  * Request b's tokens are rows starts[b] .. starts[b + 1] - 1 of the step
  * (starts [batch + 1], the exclusive sums of the positive new_lens).  It gets
  * them if they end at or below num_tokens and fit its table row and, where
@@ -562,7 +564,8 @@ int tq_paged_plan(const int *kv_lens, const int *new_lens, int batch, int *block
  *   2 i + 1) when interleaved; the angle is formed and reduced in 64 bits.
  * One rounding, at the output.  Rows of negative positions are left as they
  * are.  head_dim a multiple of 32 up to 256; inv_freq f32 [rot_dim / 2].
- * num_heads or num_kv_heads may be 0 (then its pointers are not read). */
+ * num_heads or num_kv_heads may be 0 (then its pointers are not read).
+ * tokens below 2^26. */
 int tq_qk_norm_rope(const void *q, long long q_stride, const void *k, long long k_stride, int dtype,
                     const int *positions, int tokens, int num_heads, int num_kv_heads,
                     int head_dim, const float *inv_freq, int rot_dim, int interleaved,
@@ -575,7 +578,8 @@ int tq_qk_norm_rope(const void *q, long long q_stride, const void *k, long long 
  * [tokens], the codes and scales of tq_polar_quantize; rows whose slot names
  * no token are skipped.  signs non-null (with norms and sign_matrix, head_dim
  * 64, 128 or 256, outlier_blocks 0): the keys' QJL sketch too
- * (tq_qjl_cache_sketch).  The slots that name a token are distinct. */
+ * (tq_qjl_cache_sketch).  The slots that name a token are distinct.  tokens *
+ * num_kv_heads * head_dim / 32 below 2^30. */
 int tq_paged_store(const void *k, long long k_stride, const void *v, long long v_stride, int dtype,
                    const long long *slots, int tokens, uint8_t *k_indices, uint16_t *k_scales,
                    uint8_t *v_indices, uint16_t *v_scales, uint8_t *signs, uint16_t *norms,
@@ -585,7 +589,8 @@ int tq_paged_store(const void *k, long long k_stride, const void *v, long long v
 
 /* The records of slots [tokens] back as activations: k_out and v_out
  * [tokens][num_kv_heads][head_dim] in out_dtype (tq_polar_dequantize's
- * values); rows whose slot names no token are left as they are. */
+ * values); rows whose slot names no token are left as they are.  Tokens as
+ * many as tq_paged_store takes. */
 int tq_paged_load(const uint8_t *k_indices, const uint16_t *k_scales, const uint8_t *v_indices,
                   const uint16_t *v_scales, const long long *slots, int tokens, long long num_pages,
                   int num_kv_heads, int page_size, int head_dim, int bits, size_t outlier_blocks,
@@ -593,7 +598,8 @@ int tq_paged_load(const uint8_t *k_indices, const uint16_t *k_scales, const uint
 
 /* Attention of one new token per request over its pages: q and out [batch]
  * [num_heads][head_dim]; request b attends to its first kv_lens[b] tokens
- * (device lengths, clamped to 0 .. max_kv_len <= table_width * page_size).
+ * (device lengths, clamped to 0 .. max_kv_len <= table_width * page_size, at
+ * most 2^27).  head_dim 32, 64, 128 or 256 (TQ: not 32); batch up to 65,535.
  * Arguments otherwise as tq_cache_decode_attention; signs non-null selects
  * TQ with the projection of the query formed in the launch from sign_matrix.
  * A table entry outside [0, num_pages) holds no tokens: its positions are

@@ -71,6 +71,13 @@ def test_store_refuses(kw, code):
     assert _store(**kw) == code
 
 
+@pytest.mark.parametrize("call", ["store", "decode"])
+@pytest.mark.parametrize("offset", [1, 4, 8])
+def test_sign_pools_start_on_a_16_byte_boundary(call, offset):
+    kw = dict(signs=0x1000 + offset, norms=P, rm=P, ob=0)
+    assert (_store(**kw) if call == "store" else _decode(**kw)) == 6
+
+
 def test_store_of_nothing_is_nothing():
     assert _store(tokens=0, k=None) == 0
 

@@ -436,9 +436,8 @@ extern "C" int tq_paged_decode_attention(const void *q, int q_dtype, const uint8
   if (!q || !out || !kv_lens || !k_indices || !k_scales || !v_indices || !v_scales || (max_kv_len && !block_table) ||
       (signs && (!norms || !sign_matrix)) || !workspace)
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "null pointer");
-  for (const void *p : {(const void *)k_indices, (const void *)v_indices, (const void *)k_scales, (const void *)v_scales})
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
-      return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "code and scale pools start on 16-byte boundaries");
+  rc = tqh::check_pools({k_indices, v_indices, k_scales, v_scales, signs});
+  if (rc) return rc;
   const WsLayout w = ws_layout(batch, num_heads, num_kv_heads, head_dim, max_kv_len);
   if (workspace_bytes < w.total)
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "workspace too small: %zu < %zu", workspace_bytes, w.total);

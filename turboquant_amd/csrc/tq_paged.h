@@ -1,7 +1,10 @@
-// tq_paged.h -- what the entries over a paged cache share on the host.
+// tq_paged.h -- what the entries over a paged cache share: the checks of their
+// arguments, and the store of large outputs.
 #pragma once
 
 #include "tq_common.h"
+
+#include <initializer_list>
 
 namespace tqh {
 
@@ -31,10 +34,19 @@ inline int check_pages(long long num_pages, int num_kv_heads, int page_size, int
   return TQ_OK;
 }
 
+// Refuses a pool that does not start on a 16-byte boundary (null: there is none).
+inline int check_pools(std::initializer_list<const void *> pools) {
+  for (const void *p : pools)
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+      return fail(TQ_ERR_INVALID_ARGUMENT, "code, scale and sign pools start on 16-byte boundaries");
+  return TQ_OK;
+}
+
 // Whether rows of `stride` elements of `size` bytes from p start on 16-byte boundaries.
 inline bool rows_aligned(const void *p, long long stride, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
 }
+
 // A 16-byte store; `through`: with no wish to find it in a cache again.  Output
 // of more than kThroughBytes, the size of the dies' L2s, is not there when it is
 // read, and its lines push out what the kernel still reads (8,192 tokens' heads

@@ -220,8 +220,6 @@ float decode_factor() {
   return inv * sq;  // fl(fl(1/sqrt 32) * sqrt 32) (wht_tensor.rs:28-41)
 }
 
-bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-
 // f(integral_constant DT) for a valid element type
 template <class F>
 void by_type(int dt, F &&f) {
@@ -239,8 +237,8 @@ extern "C" int tq_paged_store(const void *k, long long k_stride, const void *v, 
                               int head_dim, int bits, size_t outlier_blocks, int norm_mode, hipStream_t stream) {
   StoreArgs a{};
   tqh::PolarCodec codec;
-  const int rc = tqh::check_pages(num_pages, num_kv_heads, page_size, head_dim, bits, outlier_blocks, norm_mode,
-                                  a.pages.shift, codec);
+  int rc = tqh::check_pages(num_pages, num_kv_heads, page_size, head_dim, bits, outlier_blocks, norm_mode,
+                            a.pages.shift, codec);
   if (rc) return rc;
   if (!tqh::valid_dtype(dtype)) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
   if (tokens < 0) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "negative tokens");
@@ -254,8 +252,8 @@ extern "C" int tq_paged_store(const void *k, long long k_stride, const void *v, 
   if (tokens == 0 || num_pages == 0) return TQ_OK;
   if (!k || !v || !slots || !k_indices || !k_scales || !v_indices || !v_scales || (signs && (!norms || !sign_matrix)))
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "null pointer");
-  if (!aligned16(k_indices) || !aligned16(v_indices) || !aligned16(k_scales) || !aligned16(v_scales))
-    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "code and scale pools start on 16-byte boundaries");
+  rc = tqh::check_pools({k_indices, v_indices, k_scales, v_scales, signs});
+  if (rc) return rc;
   const long long lanes = (long long)tokens * num_kv_heads * (head_dim / 32);
   if (lanes >= 1ll << 30) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "too many tokens in one call");
   const int size = tqh::dtype_size(dtype);
@@ -324,17 +322,18 @@ extern "C" int tq_paged_load(const uint8_t *k_indices, const uint16_t *k_scales,
                              int norm_mode, void *k_out, void *v_out, int out_dtype, hipStream_t stream) {
   LoadArgs a{};
   tqh::PolarCodec codec;
-  const int rc = tqh::check_pages(num_pages, num_kv_heads, page_size, head_dim, bits, outlier_blocks, norm_mode,
-                                  a.pages.shift, codec);
+  int rc = tqh::check_pages(num_pages, num_kv_heads, page_size, head_dim, bits, outlier_blocks, norm_mode,
+                            a.pages.shift, codec);
   if (rc) return rc;
   if (!tqh::valid_dtype(out_dtype)) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "unknown dtype %d", out_dtype);
   if (tokens < 0) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "negative tokens");
   if (tokens == 0 || num_pages == 0) return TQ_OK;
   if (!slots || !k_indices || !k_scales || !v_indices || !v_scales || !k_out || !v_out)
     return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "null pointer");
-  if (!aligned16(k_indices) || !aligned16(v_indices) || !aligned16(k_scales) || !aligned16(v_scales) ||
-      !aligned16(k_out) || !aligned16(v_out))
-    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "pools and outputs start on 16-byte boundaries");
+  rc = tqh::check_pools({k_indices, v_indices, k_scales, v_scales});
+  if (rc) return rc;
+  if (!tqh::rows_aligned(k_out, 0, 1) || !tqh::rows_aligned(v_out, 0, 1))
+    return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "outputs start on 16-byte boundaries");
   const long long lanes = (long long)tokens * num_kv_heads * (head_dim / 32);
   if (lanes >= 1ll << 30) return tqh::fail(TQ_ERR_INVALID_ARGUMENT, "too many tokens in one call");
   a.pages.slots = slots;
