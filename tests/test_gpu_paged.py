@@ -713,6 +713,29 @@ def test_a_captured_step_replays(tq):
         assert caches[0].kv_lens.tolist() == caches[1].kv_lens.tolist()
 
 
+def test_a_workspace_is_made_outside_of_a_capture_and_stays(tq, monkeypatch):
+    """A graph's workspace is not given back when another number of heads asks for its own."""
+    cache = tq.PagedCache(tq.CacheConfig(3, 64, 2, 1), 64, 2, 512, 16)
+    k = torch.randn(700, 2, 64, device="cuda")
+    cache.store(0, cache.plan(i32(450, 250), 700), k, k.flip(0))
+    few, many = torch.randn(2, 4, 64, device="cuda"), torch.randn(2, 16, 64, device="cuda")
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            cache.attend(0, few, 0.125)
+    ref = cache.attend(0, few, 0.125)
+    held = cache._ws[4].buf.data_ptr()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = cache.attend(0, few, 0.125)
+    for _ in range(3):
+        other = cache.attend(0, many, 0.125)
+        graph.replay()
+        assert torch.equal(out, ref) and cache._ws[4].buf.data_ptr() == held
+        assert torch.equal(other, cache.attend(0, many, 0.125))
+
+
 def test_on_another_stream(tq):
     """The calls run on the current stream: work that it waits for is seen."""
     d, hk, n = 64, 1, 300

@@ -299,7 +299,9 @@ class PagedCache:
         out = cache.step(layer, plan, q, k, v, scale, rope)   # decode, each layer
 
     Calls are ordered on one stream; graphs captured from them share the cache
-    and its workspace, and are replayed in order."""
+    and its workspaces, and are replayed in order.  The first `attend` or `step`
+    with a number of heads makes its workspace, outside of a capture; it stays
+    for as long as the cache, which outlives its graphs."""
 
     def __init__(self, config: CacheConfig, num_pages: int, max_requests: int, max_kv_len: int, page_size: int = 64,
                  qjl: bool = False, device="cuda"):
@@ -323,7 +325,7 @@ class PagedCache:
         if qjl:
             from . import qjl_sign_matrix
             self.sign_matrix = qjl_sign_matrix(config.head_dim, DEFAULT_QJL_SEED, device)
-        self._ws = None
+        self._ws = {}  # by number of heads; none is replaced, graphs hold their addresses
 
     def plan(self, new_lens: torch.Tensor, num_tokens: int) -> PagePlan:
         """One step's pages and slots (`paged_plan`); the cache's lengths, table
@@ -348,13 +350,17 @@ class PagedCache:
         """q [max_requests, heads, head_dim], a row per request, over all of its tokens."""
         if q.dim() != 3 or q.shape[0] != self.max_requests:
             raise ValueError(f"q must be [{self.max_requests}, heads, head_dim]")
-        if self._ws is None or self._ws.shape[1] < q.shape[1]:
+        ws = self._ws.get(q.shape[1])
+        if ws is None:
             from . import AttentionWorkspace
-            self._ws = AttentionWorkspace(self.max_requests, q.shape[1], self.config.num_kv_heads,
-                                          self.config.head_dim, self.max_kv_len, q.device)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"the first call with {q.shape[1]} heads makes a workspace: call once before the "
+                                   "capture")
+            ws = self._ws[q.shape[1]] = AttentionWorkspace(self.max_requests, q.shape[1], self.config.num_kv_heads,
+                                                           self.config.head_dim, self.max_kv_len, q.device)
         bits, outlier_blocks, norm_mode = self._mode()
         return paged_decode_attention(q, self.layers[layer], self.block_table, self.kv_lens, bits, self.max_kv_len,
-                                      softmax_scale, self._ws, outlier_blocks, norm_mode, self.sign_matrix, out_dtype)
+                                      softmax_scale, ws, outlier_blocks, norm_mode, self.sign_matrix, out_dtype)
 
     def step(self, layer: int, plan: PagePlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
              softmax_scale: float, rope: Optional[QkNormRope] = None) -> torch.Tensor:
