@@ -183,14 +183,19 @@ struct DecCfg {
   static constexpr int NPAIR = 1 << (CPR * BITS);
   static constexpr int SW4 = (NQB + 3) / 4;      // QJL: sign words per lane and tile
   static constexpr int TPL = TPW / 64;           // V-scale tokens per lane
-  static constexpr bool QA_REGS = QG * KJ <= 8;  // query operands in registers (else LDS)
+  // query operands in registers, else LDS (quads of 8 heads of 256, whose
+  // records' words take the registers)
+  static constexpr bool QA_REGS = QG * KJ <= 8 && !(QUAD && NQB == 8 && HG == 8);
   // LDS carve (32-bit words)
   static constexpr int OFF_PAIR = 0;                                  // uint2 [NPAIR]: pairs, or quads
   static constexpr int OFF_NIB = OFF_PAIR + 2 * NPAIR;                // QJL uint2 [16]
   // the key-pass query operands, u32x4 [QG*KJ][64] (read per instruction,
   // or by QA_REGS configurations into registers at each chunk's K pass)
   static constexpr int OFF_QA = (OFF_NIB + (QJL ? 32 : 0) + 3) & ~3;
-  static constexpr int OFF_W = OFF_QA + QG * KJ * 64 * 4;
+  // QUAD with QJL: the correction's operands, u32x4 [4 * SW4][64], read at each
+  // chunk's K pass (in registers throughout they spill: 138 -> 114 us)
+  static constexpr int OFF_RA = OFF_QA + QG * KJ * 64 * 4;
+  static constexpr int OFF_W = OFF_RA + (QUAD && QJL ? 4 * SW4 * 64 * 4 : 0);
   // the query setup lives in the wave staging area until the K pass starts
   static constexpr int OFF_Q = OFF_W;                                 // [HG][HD] scaled rotated query
   static constexpr int OFF_QMAX = OFF_Q + HG * HD;                    // [HG][NQB] block max |qt|
@@ -211,7 +216,13 @@ struct DecCfg {
   static constexpr int WM = WC + HG * HD;
   static constexpr int WSTAGE = (WM + 3 * HG + 1 + 3) & ~3;
   static constexpr int TOTAL = OFF_W + WAVES * WSTAGE;
-  static constexpr int MERGE_LDS = merge_lds(WAVES);
+  // QUAD: the merge's scratch lies where the table was (8 heads of 64: two workgroups a
+  // compute unit instead of one, 142 -> 109 us for 120 sequences of up to 8,192 tokens)
+  static constexpr int MERGE_LDS = QUAD ? 0 : merge_lds(WAVES);
+  static constexpr int QUAD_WPE = NQB <= 4 && TOTAL * 4 + 512 <= 80 * 1024 ? 4 : 2;  // waves a SIMD: heads of 256 need more than 128 registers
+  // tiles of records ahead of a QUAD kernel's passes, and whether its LDS is there
+  static constexpr int QUAD_LA = !QA_REGS || (QUAD_WPE == 4 && (NQB == 4 || (QJL && HG == 8))) ? 1 : 2;
+  static constexpr bool QUAD_FITS = TOTAL * 4 + 512 <= 160 * 1024;
   static_assert(SETUP_END <= TOTAL, "the query setup fits the staging area");
   static_assert(HG >= 1 && HG <= 8, "heads per group");
   static_assert(TPW % 64 == 0, "whole V-scale loads per lane");
@@ -282,12 +293,10 @@ __device__ __forceinline__ void buf_words(uint32_t (&w)[N], __amdgpu_buffer_rsrc
 // load per chunk, MAXC chunks per lane in one latency round, an online
 // update beyond); the W sets meet once in LDS.
 // ---------------------------------------------------------------------------
+// (s_ma: W * 256 floats of LDS on a 16-byte boundary, s_mml: W * 8 * 2)
 template <int HD, int W>
-__device__ void merge_heads(const AttnArgs &a, int b, int g, int nchunks) {
+__device__ __forceinline__ void merge_heads(const AttnArgs &a, int b, int g, int nchunks, float *s_ma, float *s_mml) {
   constexpr int MAXC = 64 / W;
-  __shared__ __attribute__((aligned(16))) float s_ma[W * 256];
-  __shared__ float s_mml[W * 8 * 2];
-  static_assert(sizeof(s_ma) + sizeof(s_mml) == merge_lds(W), "merge scratch");
   const int tid = threadIdx.x, part = tid >> 6, quad = tid & 63;
   const long long bh0 = (long long)b * a.num_heads + (long long)g * a.nr;
   const int outs = a.nr * HD;

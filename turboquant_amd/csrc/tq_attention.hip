@@ -44,7 +44,8 @@ __global__ __launch_bounds__(256) void stream_merge_kernel(AttnArgs a) {
   const int len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.max_len) : a.single_len;
   const int nchunks = (len + a.chunk - 1) / a.chunk;
   if (nchunks == 0) return;
-  merge_heads<HD, 4>(a, b, g, (nchunks + a.cpr - 1) / a.cpr);
+  __shared__ __attribute__((aligned(16))) float s_merge[merge_lds(4) / 4];
+  merge_heads<HD, 4>(a, b, g, (nchunks + a.cpr - 1) / a.cpr, s_merge, s_merge + 4 * 256);
 }
 
 __global__ void fill_zero_kernel(int *p, long long n) {

@@ -277,7 +277,7 @@ template <class C, bool INLINE_MERGE, bool GRID, bool MULTI, bool PROJ = false, 
 #ifndef TQ_DECODE_WPE
 #define TQ_DECODE_WPE 2
 #endif
-__global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void stream_decode_kernel(const uint8_t *k_idx, const uint8_t *v_idx,
+__global__ __launch_bounds__(C::THREADS, C::QUAD ? C::QUAD_WPE : TQ_DECODE_WPE) void stream_decode_kernel(const uint8_t *k_idx, const uint8_t *v_idx,
                                                                const uint16_t *k_sc, const uint16_t *v_sc,
                                                                long long seq_stride, long long kv_head_stride,
                                                                int len_hint, AttnArgs a,
@@ -315,7 +315,10 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
   // pairs) and the vector unit (49 %); quads take 128 registers, four waves a
   // SIMD instead of two.  128 ragged sequences of up to 8,192 tokens, 16 over 8
   // heads, 238 -> 172 us, 64 117 -> 79, 16 of up to 16,384, 32 over 8 heads,
-  // 59.7 -> 51.8.
+  // 59.7 -> 51.8.  Heads of 256, and 8 of 128 a KV head, take up to 256 registers
+  // and two waves a SIMD as with pairs, whose kernels spill: 64 sequences, 2, 4
+  // and 8 heads of 256 over each of 4 KV heads, 227 -> 98, 259 -> 115 and 694 ->
+  // 322 us; 32 of 64 heads of 128 over 8, 192 -> 80.
   constexpr bool QUAD = C::QUAD;
   static_assert(!QUAD || (BITS == 3 && MULTI && PAGED && !GRID), "quads: range launches over 3-bit pages");
   constexpr float kQuadScale = QUAD ? (C::CB == 3 ? 1.8351183f : 1.8351586f) : 1.f;
@@ -327,6 +330,7 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
   float *s_qsum = lds + C::OFF_QSUM - LSH;
   uint2 *s_nib = reinterpret_cast<uint2 *>(lds + C::OFF_NIB);
   u32x4 *s_qa = reinterpret_cast<u32x4 *>(lds + (GRID ? 0 : C::OFF_QA));
+  u32x4 *const s_ra = reinterpret_cast<u32x4 *>(lds + (QUAD ? C::OFF_RA : 0));  // QUAD: the correction's operands
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: the wave's scalar offsets
@@ -725,9 +729,10 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
 #endif
   // LA0 K tiles go out with the first chunk's prologue (more would hold the
   // waves at issue before their setup), LA during the K passes
-  // QUAD: two tiles ahead (128 registers, four waves a SIMD; four ahead spill
-  // and measured the same, 78 us against 82 at 64 sequences)
-  constexpr int LA = dmin(QUAD ? 2 : (MULTI ? TQ_DECODE_LOOKAHEAD_MULTI : TQ_DECODE_LOOKAHEAD_PASS), NKT);
+  // QUAD: two tiles ahead, or one where two spill (64 ragged sequences of up to
+  // 8,192 tokens of 128, QJL, 16 heads over 8 KV heads 114 -> 93 us, 32 over 8
+  // 131 -> 116; 8 heads of 256 a KV head, PQO, 416 -> 322).  Four spill too.
+  constexpr int LA = dmin(QUAD ? C::QUAD_LA : (MULTI ? TQ_DECODE_LOOKAHEAD_MULTI : TQ_DECODE_LOOKAHEAD_PASS), NKT);
   constexpr int LA0 = MULTI ? LA : dmin(C::LOOKAHEAD, LA);
   constexpr int VP_NEXT = NVP >= 2 ? NVP - 2 : 0;
   auto issue_first = [&](uint32_t tw0, int n) {
@@ -1024,6 +1029,7 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
     const int hl = (2 * r) % HPM + u;
 #pragma unroll
     for (int s = 0; s < 4 * C::SW4; s++) {
+      if (QUAD && s % C::WAVES != wave) continue;  // a wave an operand, through LDS
       const int wi = (s >> 2) * 4 + lg, sb = s & 3;
       u32x4 val = {0u, 0u, 0u, 0u};
       if (hl < nh && wi < NQB) {
@@ -1038,7 +1044,8 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
         }
         val = u32x4{wv[0], wv[1], wv[2], wv[3]};
       }
-      ra[s] = val;
+      if constexpr (QUAD) s_ra[s * 64 + lane] = val;
+      else ra[s] = val;
     }
   }
   // the query setup is dead from here: the staging area it lives in is the waves' own
@@ -1091,6 +1098,10 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
     if constexpr (MULTI) asm volatile("" : "+v"(qoff));
 #pragma unroll
     for (int k = 0; k < QG * KJA; k++) qa[k] = s_qa[k * 64 + qoff];
+    if constexpr (QUAD && C::QJL) {
+#pragma unroll
+      for (int k = 0; k < 4 * C::SW4; k++) ra[k] = s_ra[k * 64 + qoff];
+    }
   }
   float sc[NKT][NS];
 #pragma unroll
@@ -1134,7 +1145,7 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
       for (int s = 0; s < 4 * C::SW4; s++) {
         const uint32_t byte = (sgw[i][s >> 2] >> (8 * (s & 3))) & 0xffu;
         const uint2 n0 = s_nib[byte & 15u], n1 = s_nib[byte >> 4];
-        dq = mfma(ra[s], u32x4{n0.x, n0.y, n1.x, n1.y}, dq);
+        dq = mfma(QUAD && !QAR ? s_ra[s * 64 + lane] : ra[s], u32x4{n0.x, n0.y, n1.x, n1.y}, dq);
       }
     }
     // lane (token l16, row group lg): rows (qbl, head hl0 + u, part)
@@ -1543,7 +1554,13 @@ __global__ __launch_bounds__(C::THREADS, C::QUAD ? 4 : TQ_DECODE_WPE) void strea
     }
   } else if (s_flag) {
     if constexpr (INLINE_MERGE) {
-      merge_heads<HD, C::WAVES>(a, b, g, nparts);
+      if constexpr (QUAD) {  // the codebook has been read
+        static_assert(2 * C::NPAIR >= merge_lds(C::WAVES) / 4, "the merge's scratch fits the table");
+        merge_heads<HD, C::WAVES>(a, b, g, nparts, lds, lds + C::WAVES * 256);
+      } else {
+        __shared__ __attribute__((aligned(16))) float s_merge[merge_lds(C::WAVES) / 4];
+        merge_heads<HD, C::WAVES>(a, b, g, nparts, s_merge, s_merge + C::WAVES * 256);
+      }
       if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
@@ -1718,7 +1735,7 @@ void launch_stream_cfg(AttnArgs &a, dim3 grid, hipStream_t st, X *ap) {
   using C4 = StreamCfg4<BITS, MODE, NQB, HG>;
   using C64 = StreamCfg64<BITS, MODE, NQB, HG>;
   using CQ = StreamCfgQuad<BITS, MODE, NQB, HG>;
-  if constexpr (std::is_same_v<X, PageArgs> && BITS == 3 && CQ::TOTAL * 4 + CQ::MERGE_LDS + 512 <= 80 * 1024) {
+  if constexpr (std::is_same_v<X, PageArgs> && BITS == 3 && CQ::QUAD_FITS) {
     // range launches on the MaxNorm codebook with 16-bit results
     const long long tasks = (long long)((a.max_len + C4::CHUNK - 1) / C4::CHUNK) * grid.y * grid.z;
     if (tasks > 3ll * device_cus() && a.out_dtype != kF32 && !a.cb_args) return launch_stream_c<CQ, INLINE>(a, grid, st, ap);
